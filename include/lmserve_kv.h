@@ -288,6 +288,95 @@ int lms_rope_and_cache(const void* query, const void* key, const void* value,
                        int64_t num_slots, int64_t max_position, void* stream);
 
 /*
+ * Norm of every query and key head, rotary position embedding and (optionally) the paged cache
+ * write of one layer in one launch: lms_rope_and_cache for layers that normalise each head of Q
+ * and K before they rotate it.  For every head x of Q and K, with w = query_weight / key_weight
+ * ([head_dim], shared by the heads):
+ *   n = x * w / sqrt(mean(x^2) + eps),   then the two lines of lms_rope_and_cache on n,
+ * evaluated in fp32 and rounded once.  Arguments, layouts and the slot < 0 padding rule are those
+ * of lms_rope_and_cache, with two differences: max_position and (with a cache) num_slots are
+ * required and always enforced - a token whose position is outside the table gets no rotated Q
+ * and no K, one whose slot is outside the cache no cache row; the debug checks report it - and
+ * head_dim is a multiple of 16 up to 512.  (The reference has no such model; the call takes the
+ * place of rotary_pos_emb at runtime/worker/llm_worker/models/llama.py:156-167.)
+ */
+int lms_qk_norm_rope_and_cache(const void* query, const void* key, const void* value,
+                               int64_t query_token_stride, int64_t key_token_stride,
+                               int64_t value_token_stride, const void* query_weight,
+                               const void* key_weight, double eps, const void* positions,
+                               int32_t positions_are_int64, const void* cos_sin_cache,
+                               int64_t cos_sin_row_stride, void* q_out,
+                               int64_t q_out_token_stride, void* k_out,
+                               int64_t k_out_token_stride, void* key_cache,
+                               void* value_cache, int64_t block_stride, int64_t slot_stride,
+                               const int64_t* slot_mapping, int64_t num_tokens,
+                               int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                               int32_t dtype, int32_t block_size, int64_t num_slots,
+                               int64_t max_position, void* stream);
+
+/*
+ * Attention of a batch over its pages of one layer's cache - the call of
+ *   prefill_wrapper.run / decode_wrapper.run   runtime/worker/llm_worker/models/layers/attention.py:87-106
+ * (flashinfer's paged wrappers) on the index arrays lms_build_step_indices leaves on the device,
+ * without a planning step: every launch derives its work from those arrays on the device, so a
+ * captured call follows their contents from replay to replay.
+ *
+ * query [num_tokens, num_heads, head_dim] (token stride in bytes, heads dense), out likewise, lse
+ * float [num_tokens, num_heads] or NULL.  Request b owns the pages
+ * kv_indices[kv_indptr[b] .. kv_indptr[b+1]), the last of them with kv_last_page_len[b] keys, and
+ * the tokens [qo_indptr[b], qo_indptr[b+1]) (qo_indptr == NULL: token b alone, num_tokens ==
+ * num_requests).  Its n tokens are the last n of its len keys: with causal != 0 the i-th reads the
+ * keys j <= len - n + i, else all.  Query head h reads key head h / (num_heads / num_kv_heads).
+ *   s_j = scale * q.k_j,  out = sum_j exp(s_j - lse) v_j,  lse = log sum_j exp(s_j)
+ * A row without any key gives out = 0 and lse = -inf; tokens outside [qo_indptr[0],
+ * qo_indptr[num_requests]) are left as they are.
+ *
+ * Shared prefixes (num_groups > 0): the requests [group_indptr[g], group_indptr[g+1])
+ * (group_indptr == NULL: num_groups == 1, all requests) read, before their own keys, every key of
+ * the pages prefix_indices[prefix_indptr[g] .. prefix_indptr[g+1]) (last page:
+ * prefix_last_page_len[g] keys).  The result is that of a page table with the prefix in front of
+ * each request's own pages; the prefix's keys are read once for all rows of the group.  A request
+ * outside every group has no prefix.
+ *
+ * Pages: key / value cache with block_stride bytes between pages and slot_stride bytes between
+ * the keys of a page (the interleaved cache of lms_reshape_and_cache or two separate ones).  Page
+ * numbers outside [0, num_blocks) and table places outside [0, num_*_indices) are never
+ * dereferenced: such keys read as zeros, and the debug checks report the page.
+ * `workspace`: lms_attention_workspace_bytes(args) bytes of device memory, 256-byte aligned, that
+ * no other call in flight uses; its contents need not be kept or cleared.  The size depends on
+ * the counts in `args` alone, not on the arrays' contents.
+ * dtype 0 = fp16, 1 = bf16; head_dim a multiple of 8 up to 256.
+ */
+typedef struct lms_attention_args {
+  const void* query;
+  void* out;
+  float* lse;
+  const void* key_cache;
+  const void* value_cache;
+  int64_t query_token_stride, out_token_stride;
+  int64_t block_stride, slot_stride;
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  const int32_t* kv_last_page_len;
+  int64_t num_kv_indices;
+  const int32_t* qo_indptr;
+  const int32_t* prefix_indptr;
+  const int32_t* prefix_indices;
+  const int32_t* prefix_last_page_len;
+  int64_t num_prefix_indices;
+  const int32_t* group_indptr;
+  int64_t num_tokens, num_requests, num_groups, num_blocks;
+  int64_t num_heads, num_kv_heads, head_dim, block_size;
+  int64_t dtype, causal;
+  double scale;
+  void* workspace;
+  int64_t workspace_bytes;
+} lms_attention_args;
+/* Bytes, or a negative status for arguments the call would refuse. */
+int64_t lms_attention_workspace_bytes(const lms_attention_args* args);
+int lms_paged_attention(const lms_attention_args* args, void* stream);
+
+/*
  * Copy-on-write block copy — replaces
  *   copy_blocks               runtime/worker/llm_worker/ops/cache_ops.py:8-36
  *   copy_blocks_kernel        runtime/worker/llm_worker/ops/triton/cache_kernels.py:5-36

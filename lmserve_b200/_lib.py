@@ -6,7 +6,7 @@ symbol the header declares, importing this module's ``lib()`` raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_int, c_int32, c_int64, c_void_p, POINTER
+from ctypes import c_char_p, c_double, c_int, c_int32, c_int64, c_void_p, POINTER
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "liblmserve_kv.so"
@@ -82,6 +82,13 @@ SIGNATURES = {
         c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,
         c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64,
         c_void_p]),
+    "lms_qk_norm_rope_and_cache": (c_int, [
+        c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_double,
+        c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+        c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,
+        c_int64, c_int64, c_void_p]),
+    "lms_attention_workspace_bytes": (c_int64, [c_void_p]),
+    "lms_paged_attention": (c_int, [c_void_p, c_void_p]),
     "lms_build_step_indices": (c_int, [
         c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64,
         c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -141,7 +148,7 @@ def lib() -> ctypes.CDLL:
         return _lib
     if not LIB_PATH.exists():
         raise ImportError(
-            f"{LIB_PATH} is missing: build it with `python -m lmserve_b200.build` "
+            f"{LIB_PATH} is missing: build it with `python lmserve_b200/build.py` "
             "(nvcc, sm_100a). There is no CPU or PyTorch fallback for the cache ops.")
     handle = ctypes.CDLL(str(LIB_PATH))
     for name, (restype, argtypes) in SIGNATURES.items():

@@ -7,7 +7,7 @@ bound from cgo / JNI / FFI) without PyTorch.
 ``build_packer()`` compiles the small CPython extension ``_packer`` (``csrc/packer.c``, gcc)
 that packs a step's request list for ``lms_build_step_indices``; it is host code only.
 
-Run ``python -m lmserve_b200.build`` to (re)build both; ``build_library()`` and
+Run ``python lmserve_b200/build.py`` to (re)build both; ``build_library()`` and
 ``build_packer()`` are what ``__graft_entry__.build()`` calls.
 """
 from __future__ import annotations
@@ -22,7 +22,8 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_NAME = "liblmserve_kv.so"
 LIB_PATH = PKG_DIR / LIB_NAME
-SOURCES = ["capi.cu", "write_rows.cu", "chunk_copy.cu", "rope_cache.cu", "step_indices.cu"]
+SOURCES = ["capi.cu", "write_rows.cu", "chunk_copy.cu", "rope_cache.cu", "step_indices.cu",
+           "qk_norm_rope.cu", "paged_attention.cu"]
 HEADERS = ["kv_common.cuh", "kernels.cuh"]
 PUBLIC_HEADER = PKG_DIR.parent / "include" / "lmserve_kv.h"
 

@@ -360,6 +360,72 @@ int static_table(StaticTable** out) {
   return LMS_OK;
 }
 
+// Validates the arguments of an attention call and fills the kernel parameter block (without the
+// workspace, the error record and the checks flag).
+int attention_params(const lms_attention_args* a, AttentionParams* out, bool* empty) {
+  *empty = false;
+  if (!a) return LMS_ERR_NULL;
+  constexpr int64_t kMax = 0x7fffffffll;
+  if (a->num_tokens < 0 || a->num_tokens > kMax || a->num_requests < 0 || a->num_requests >= kMax ||
+      a->num_groups < 0 || a->num_groups >= kMax || a->num_blocks < 0 || a->num_blocks > kMax ||
+      a->num_kv_indices < 0 || a->num_kv_indices > kMax || a->num_prefix_indices < 0 ||
+      a->num_prefix_indices > kMax || a->num_heads <= 0 || a->num_heads > 65535 ||
+      a->num_kv_heads <= 0 || a->num_heads % a->num_kv_heads != 0 || a->head_dim <= 0 ||
+      a->block_size <= 0 || a->block_size > (1 << 20) || (a->dtype != 0 && a->dtype != 1) ||
+      !(a->scale >= -1e30 && a->scale <= 1e30))
+    return LMS_ERR_RANGE;
+  if (a->head_dim % 8 != 0 || a->head_dim > 256) return LMS_ERR_UNSUPPORTED;
+  if (a->qo_indptr == nullptr && a->num_tokens != a->num_requests) return LMS_ERR_RANGE;
+  if (a->num_groups > 1 && a->group_indptr == nullptr) return LMS_ERR_NULL;
+  if (a->num_tokens == 0 || a->num_requests == 0) {
+    *empty = true;
+    return LMS_OK;
+  }
+  if (!a->query || !a->out || !a->kv_indptr || !a->kv_last_page_len ||
+      (a->num_kv_indices > 0 && !a->kv_indices) ||
+      (a->num_blocks > 0 && (!a->key_cache || !a->value_cache)))
+    return LMS_ERR_NULL;
+  if (a->num_groups > 0 && (!a->prefix_indptr || !a->prefix_last_page_len ||
+                            (a->num_prefix_indices > 0 && !a->prefix_indices)))
+    return LMS_ERR_NULL;
+  if (!ptr16(a->query) || !ptr16(a->out) || !ptr16(a->key_cache) || !ptr16(a->value_cache) ||
+      !mult16(a->query_token_stride) || !mult16(a->out_token_stride) || !mult16(a->block_stride) ||
+      !mult16(a->slot_stride) ||
+      (((uintptr_t)a->lse | (uintptr_t)a->kv_indptr | (uintptr_t)a->kv_indices |
+        (uintptr_t)a->kv_last_page_len | (uintptr_t)a->qo_indptr | (uintptr_t)a->prefix_indptr |
+        (uintptr_t)a->prefix_indices | (uintptr_t)a->prefix_last_page_len |
+        (uintptr_t)a->group_indptr) & 3u) != 0)
+    return LMS_ERR_ALIGN;
+  AttentionParams p{};
+  p.q = (const char*)a->query;
+  p.q_tok = a->query_token_stride;
+  p.out = (char*)a->out;
+  p.o_tok = a->out_token_stride;
+  p.lse = a->lse;
+  p.kcache = (const char*)a->key_cache;
+  p.vcache = (const char*)a->value_cache;
+  p.block_stride = a->block_stride;
+  p.slot_stride = a->slot_stride;
+  p.num_blocks = a->num_blocks;
+  p.own = PageList{a->kv_indptr, a->kv_indices, a->kv_last_page_len, a->num_kv_indices};
+  if (a->num_groups > 0)
+    p.prefix = PageList{a->prefix_indptr, a->prefix_indices, a->prefix_last_page_len, a->num_prefix_indices};
+  p.qo_indptr = a->qo_indptr;
+  p.group_indptr = a->num_groups > 0 ? a->group_indptr : nullptr;
+  p.num_tokens = (int)a->num_tokens;
+  p.num_requests = (int)a->num_requests;
+  p.num_groups = (int)a->num_groups;
+  p.num_heads = (int)a->num_heads;
+  p.num_kv_heads = (int)a->num_kv_heads;
+  p.head_dim = (int)a->head_dim;
+  p.block_size = (int)a->block_size;
+  p.is_bf16 = (int)a->dtype;
+  p.causal = a->causal ? 1 : 0;
+  p.scale = (float)a->scale;
+  *out = p;
+  return LMS_OK;
+}
+
 int sm_count() {
   DeviceState* ds = nullptr;
   if (device_state(&ds) != LMS_OK) return 148;
@@ -443,6 +509,11 @@ int lms_check_device_errors(void* stream, int64_t* index, int64_t* value) {
   if (h.code == kErrBadPosition) {
     snprintf(g_cuda_msg, sizeof(g_cuda_msg), "position %lld of token %lld is outside the cos/sin cache",
              h.value, h.index);
+    return LMS_ERR_INDEX;
+  }
+  if (h.code == kErrBadPage) {
+    snprintf(g_cuda_msg, sizeof(g_cuda_msg), "entry %lld of a page table names page %lld, which the cache does not have",
+             h.index, h.value);
     return LMS_ERR_INDEX;
   }
   if (h.code == kErrWaitTimeout) {
@@ -670,6 +741,113 @@ int lms_rope_and_cache(const void* query, const void* key, const void* value,
   p.checks = g_checks.load(std::memory_order_relaxed);
   LMS_CUDA(launch_rope_cache(p, tuned(LMS_TUNE_WRITE_PDL, 1) == 1, (cudaStream_t)stream));
   g_launches.fetch_add(1, std::memory_order_relaxed);
+  return LMS_OK;
+}
+
+int lms_qk_norm_rope_and_cache(const void* query, const void* key, const void* value,
+                               int64_t query_token_stride, int64_t key_token_stride,
+                               int64_t value_token_stride, const void* query_weight,
+                               const void* key_weight, double eps, const void* positions,
+                               int32_t positions_are_int64, const void* cos_sin_cache,
+                               int64_t cos_sin_row_stride, void* q_out,
+                               int64_t q_out_token_stride, void* k_out,
+                               int64_t k_out_token_stride, void* key_cache,
+                               void* value_cache, int64_t block_stride, int64_t slot_stride,
+                               const int64_t* slot_mapping, int64_t num_tokens,
+                               int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                               int32_t dtype, int32_t block_size, int64_t num_slots,
+                               int64_t max_position, void* stream) {
+  if (num_tokens < 0 || num_tokens > 0x7fffffffll || num_heads <= 0 || num_kv_heads <= 0 ||
+      num_heads > (1 << 20) || num_kv_heads > (1 << 20) || head_dim <= 0 || num_slots < 0 ||
+      max_position < 0 || (dtype != 0 && dtype != 1) || !(eps >= 0.0) || eps > 1e30)
+    return LMS_ERR_RANGE;
+  if (head_dim % 16 != 0 || head_dim > 512) return LMS_ERR_UNSUPPORTED;
+  if (num_tokens == 0) return LMS_OK;
+  const bool cached = key_cache != nullptr || value_cache != nullptr;
+  if (!query || !key || !query_weight || !key_weight || !positions || !cos_sin_cache || !q_out)
+    return LMS_ERR_NULL;
+  if (cached && (!key_cache || !value_cache || !value || !slot_mapping)) return LMS_ERR_NULL;
+  if (cached && block_size <= 0) return LMS_ERR_RANGE;
+  if (!ptr16(query) || !ptr16(key) || !ptr16(query_weight) || !ptr16(key_weight) ||
+      !ptr16(cos_sin_cache) || !ptr16(q_out) || !ptr16(k_out) || !mult16(query_token_stride) ||
+      !mult16(key_token_stride) || !mult16(cos_sin_row_stride) || !mult16(q_out_token_stride) ||
+      !mult16(k_out_token_stride) ||
+      ((uintptr_t)positions & (positions_are_int64 ? 7u : 3u)) != 0)
+    return LMS_ERR_ALIGN;
+  if (cached && (!ptr16(value) || !ptr16(key_cache) || !ptr16(value_cache) ||
+                 !mult16(value_token_stride) || !mult16(block_stride) ||
+                 !mult16(slot_stride) || ((uintptr_t)slot_mapping & 7u) != 0))
+    return LMS_ERR_ALIGN;
+
+  DeviceState* ds = nullptr;
+  if (int rc = device_state(&ds)) return rc;
+  QkNormRopeParams p{};
+  p.q = (const char*)query;
+  p.k = (const char*)key;
+  p.v = (const char*)value;
+  p.q_tok = query_token_stride;
+  p.k_tok = key_token_stride;
+  p.v_tok = value_token_stride;
+  p.q_weight = (const char*)query_weight;
+  p.k_weight = (const char*)key_weight;
+  p.eps = (float)eps;
+  p.positions = positions;
+  p.pos64 = positions_are_int64 ? 1 : 0;
+  p.cos_sin = (const char*)cos_sin_cache;
+  p.cs_row = cos_sin_row_stride;
+  p.q_out = (char*)q_out;
+  p.qo_tok = q_out_token_stride;
+  p.k_out = (char*)k_out;
+  p.ko_tok = k_out_token_stride;
+  p.kcache = cached ? (char*)key_cache : nullptr;
+  p.vcache = cached ? (char*)value_cache : nullptr;
+  p.block_stride = block_stride;
+  p.slot_stride = slot_stride;
+  p.slots = (const long long*)slot_mapping;
+  p.num_slots = num_slots;
+  p.max_pos = max_position;
+  p.num_tokens = (int)num_tokens;
+  p.num_heads = num_heads;
+  p.num_kv_heads = num_kv_heads;
+  p.head_dim = head_dim;
+  p.block_size = cached ? block_size : 1;
+  p.is_bf16 = dtype;
+  p.err = ds->err.load(std::memory_order_relaxed);
+  p.checks = g_checks.load(std::memory_order_relaxed);
+  LMS_CUDA(launch_qk_norm_rope(p, ds->sms, tuned(LMS_TUNE_WRITE_PDL, 1) == 1, (cudaStream_t)stream));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return LMS_OK;
+}
+
+int64_t lms_attention_workspace_bytes(const lms_attention_args* args) {
+  AttentionParams p{};
+  bool empty = false;
+  if (int rc = attention_params(args, &p, &empty)) return rc;
+  if (empty) return 0;
+  DeviceState* ds = nullptr;
+  if (int rc = device_state(&ds)) return rc;
+  return attention_workspace_bytes(p, ds->sms);
+}
+
+int lms_paged_attention(const lms_attention_args* args, void* stream) {
+  AttentionParams p{};
+  bool empty = false;
+  if (int rc = attention_params(args, &p, &empty)) return rc;
+  if (empty) return LMS_OK;
+  DeviceState* ds = nullptr;
+  if (int rc = device_state(&ds)) return rc;
+  const int64_t need = attention_workspace_bytes(p, ds->sms);
+  if (need > 0) {
+    if (!args->workspace) return LMS_ERR_NULL;
+    if (((uintptr_t)args->workspace & 255u) != 0) return LMS_ERR_ALIGN;
+    if (args->workspace_bytes < need) return LMS_ERR_TOO_LARGE;
+    p.workspace = (char*)args->workspace;
+  }
+  p.err = ds->err.load(std::memory_order_relaxed);
+  p.checks = g_checks.load(std::memory_order_relaxed);
+  int launches = 0;
+  LMS_CUDA(launch_attention(p, ds->sms, tuned(LMS_TUNE_WRITE_PDL, 1) == 1, &launches, (cudaStream_t)stream));
+  g_launches.fetch_add(launches, std::memory_order_relaxed);
   return LMS_OK;
 }
 

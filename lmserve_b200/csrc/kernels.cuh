@@ -1,7 +1,7 @@
 // Parameter blocks and host-side launchers of the data-movement kernels.
 // The C ABI (capi.cu) validates arguments, fills these structs and calls the
-// launchers; the kernels themselves live in write_rows.cu, chunk_copy.cu, rope_cache.cu and
-// step_indices.cu.
+// launchers; the kernels themselves live in write_rows.cu, chunk_copy.cu, rope_cache.cu,
+// qk_norm_rope.cu, paged_attention.cu and step_indices.cu.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -21,6 +21,8 @@ enum : unsigned int {
   kWhereRope = 6,
   kWhereSelfTest = 7,
   kWhereStepIndices = 8,
+  kWhereQkNorm = 9,
+  kWhereAttention = 10,
 };
 
 // ------------------------------------------------------------ paged cache write
@@ -123,6 +125,71 @@ struct RopeParams {
 };
 
 cudaError_t launch_rope_cache(const RopeParams& p, bool pdl, cudaStream_t stream);
+
+// ------------------------------------------------------------ head norm + rotary embedding + cache write
+struct QkNormRopeParams {
+  const char* q;
+  const char* k;
+  const char* v;          // unused when there is no cache
+  long long q_tok, k_tok, v_tok;  // bytes between consecutive tokens
+  const char* q_weight;   // [head_dim] elements, shared by the query heads
+  const char* k_weight;   // [head_dim] elements, shared by the key heads
+  float eps, inv_dim;
+  const void* positions;  // int32 or int64 [T]
+  int pos64;
+  const char* cos_sin;    // [max_pos, 2 * head_dim] elements: cos row then sin row
+  long long cs_row;       // bytes between consecutive positions
+  char* q_out;
+  long long qo_tok;
+  char* k_out;            // optional rotated-K output, nullptr to skip
+  long long ko_tok;
+  char* kcache;           // nullptr (with vcache) = no cache write
+  char* vcache;
+  long long block_stride, slot_stride;
+  const long long* slots;
+  long long num_slots, max_pos;  // bounds, always checked
+  int num_tokens, num_heads, num_kv_heads, head_dim;
+  int block_size, block_shift;
+  int is_bf16;
+  ErrRecord* err;
+  int checks;
+};
+
+cudaError_t launch_qk_norm_rope(const QkNormRopeParams& p, int sms, bool pdl, cudaStream_t stream);
+
+// ------------------------------------------------------------ attention over the paged cache
+// Pages of every request (or of every group's shared prefix) in CSR form.
+struct PageList {
+  const int* indptr;    // [n + 1]
+  const int* indices;   // page numbers
+  const int* last;      // [n] keys in the last page
+  long long num_indices;
+};
+
+struct AttentionParams {
+  const char* q;          // [T, num_heads, head_dim]
+  long long q_tok;        // bytes between consecutive tokens
+  char* out;
+  long long o_tok;
+  float* lse;             // [T, num_heads], natural logarithm, or nullptr
+  const char* kcache;
+  const char* vcache;
+  long long block_stride, slot_stride;  // bytes
+  long long num_blocks;   // bound of the page numbers, always checked
+  PageList own, prefix;   // prefix.indptr == nullptr: no shared prefix
+  const int* qo_indptr;     // [B + 1], nullptr: one token a request
+  const int* group_indptr;  // [G + 1] requests of each group, nullptr: one group of all requests
+  int num_tokens, num_requests, num_groups;
+  int num_heads, num_kv_heads, head_dim, block_size;
+  int is_bf16, causal;
+  float scale;            // of q.k, natural exponent
+  char* workspace;
+  ErrRecord* err;
+  int checks;
+};
+
+long long attention_workspace_bytes(const AttentionParams& p, int sms);
+cudaError_t launch_attention(const AttentionParams& p, int sms, bool pdl, int* launches, cudaStream_t stream);
 
 // ------------------------------------------------------------ per-step index preparation
 struct StepIndexParams {

@@ -30,6 +30,7 @@ enum : unsigned int {
   kErrBadDstBlock = 3,
   kErrWaitTimeout = 4,
   kErrBadPosition = 5,
+  kErrBadPage = 6,
 };
 
 __device__ __forceinline__ void report(ErrRecord* e, unsigned int code,

@@ -279,6 +279,55 @@ static PyObject* call_plan(PyObject* self, PyObject* const* args, Py_ssize_t nar
   return PyLong_FromLong((long)run(plan, stream));
 }
 
+/* call_words(fn_address, stream, words) -> status
+ *
+ * Calls an `int fn(const void* args, void* stream)` entry point whose `args` is a structure of
+ * 8-byte fields (lms_attention_args), built here on the stack from the sequence `words`: an int is
+ * stored as a 64-bit integer or address, a float as a double, None as NULL.  With stream = None
+ * the entry point is `int64_t fn(const void* args)` (lms_attention_workspace_bytes). */
+#define CALL_WORDS_MAX 64
+typedef int64_t (*size_fn)(const void*);
+
+static PyObject* call_words(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (nargs != 3 || !(PyTuple_Check(args[2]) || PyList_Check(args[2]))) {
+    PyErr_SetString(PyExc_TypeError, "call_words(fn_address, stream, words)");
+    return NULL;
+  }
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(args[2]);
+  PyObject** items = PySequence_Fast_ITEMS(args[2]);
+  uint64_t words[CALL_WORDS_MAX];
+  if (n > CALL_WORDS_MAX) {
+    PyErr_SetString(PyExc_ValueError, "call_words: too many words");
+    return NULL;
+  }
+  void* fn = PyLong_AsVoidPtr(args[0]);
+  void* stream = args[1] == Py_None ? NULL : PyLong_AsVoidPtr(args[1]);
+  for (Py_ssize_t i = 0; i < n && !PyErr_Occurred(); ++i) {
+    if (items[i] == Py_None) {
+      words[i] = 0;
+    } else if (PyFloat_Check(items[i])) {
+      const double d = PyFloat_AS_DOUBLE(items[i]);
+      memcpy(&words[i], &d, sizeof(d));
+    } else {
+      words[i] = (uint64_t)(uintptr_t)PyLong_AsVoidPtr(items[i]); /* signed or unsigned 64 bits */
+    }
+  }
+  if (PyErr_Occurred()) return NULL;
+  if (fn == NULL) {
+    PyErr_SetString(PyExc_ValueError, "call_words: NULL function address");
+    return NULL;
+  }
+  if (args[1] == Py_None) {
+    size_fn size;
+    memcpy(&size, &fn, sizeof(size));
+    return PyLong_FromLongLong((long long)size(words));
+  }
+  plan_run_fn run;
+  memcpy(&run, &fn, sizeof(run));
+  return PyLong_FromLong((long)run(words, stream));
+}
+
 static PyMethodDef methods[] = {
     {"flatten_dict", flatten_dict, METH_VARARGS, "flatten_dict(src_to_dst, out) -> number of pairs"},
     {"flatten_entries", flatten_entries, METH_VARARGS, "flatten_entries(entries, out) -> number of pairs"},
@@ -287,6 +336,8 @@ static PyMethodDef methods[] = {
      "prefill_blocks, decode_blocks)"},
     {"call_plan", (PyCFunction)(void (*)(void))call_plan, METH_FASTCALL,
      "call_plan(fn_address, plan_handle, stream) -> status of int fn(plan, stream)"},
+    {"call_words", (PyCFunction)(void (*)(void))call_words, METH_FASTCALL,
+     "call_words(fn_address, stream, words) -> status of int fn(struct of words, stream)"},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_packer",

@@ -5,6 +5,8 @@
 does the same rotation and, in the same launch, writes the rotated K and the V rows into one
 layer's paged cache — the step that follows it in ``models/llama.py:156-167`` /
 ``models/layers/attention.py:76-85`` — so K is never materialised in between.
+``qk_norm_rotary_pos_emb`` and ``qk_norm_rotary_pos_emb_and_cache`` are the same two for layers that
+normalise every query and key head before they rotate it.
 """
 from __future__ import annotations
 
@@ -151,3 +153,94 @@ def rotary_pos_emb_and_cache(query: torch.Tensor, key: torch.Tensor, value: torc
         _launch(query, key, value, positions, cos_sin_cache, head_dim, q_out, k_out, kv_cache, slots,
                 arithmetic)
     return (q_out, k_out) if return_key else q_out
+
+
+def _check_cache(query, key, value, head_dim, kv_cache, slot_mapping):
+    """Validates the cache side of a fused rotary call; returns the slots."""
+    _require_cuda("value", value)
+    _require_cuda("kv_cache", kv_cache)
+    if value.shape != key.shape or value.dtype != key.dtype or value.stride(1) != 1:
+        raise ValueError("value must match key in shape, dtype and layout")
+    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2 or kv_cache.dtype != key.dtype:
+        raise ValueError("kv_cache must be one layer [num_blocks, 2, block_size, H, D] of the key dtype")
+    NB, _, BS, H, D = kv_cache.shape
+    if D != head_dim or H * D != key.shape[1]:
+        raise ValueError("kv_cache heads do not match key")
+    if NB and kv_cache.stride()[1:] != (BS * H * D, H * D, D, 1):
+        raise ValueError("each cache block must be contiguous")
+    slots = _slots_i64(slot_mapping, query.device)
+    if slots.numel() != query.shape[0]:
+        raise ValueError("slot_mapping must have one entry per token")
+    return slots
+
+
+def _qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps,
+             kv_cache, slot_mapping, return_key):
+    _check_inputs(query, key, positions, cos_sin_cache, head_dim)
+    dev, dtype = query.device, query.dtype
+    for n, t in (("query_weight", query_weight), ("key_weight", key_weight)):
+        _require_cuda(n, t)
+        if t.dtype != dtype or t.shape != (head_dim,) or not t.is_contiguous():
+            raise ValueError(f"{n} must be a contiguous [head_dim] vector of the query dtype")
+    for n, t in (("key", key), ("positions", positions), ("cos_sin_cache", cos_sin_cache),
+                 ("query_weight", query_weight), ("key_weight", key_weight), ("value", value),
+                 ("kv_cache", kv_cache)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{n} must be on the device of query ({dev}), got {t.device}")
+    slots = None
+    if kv_cache is not None:
+        slots = _check_cache(query, key, value, head_dim, kv_cache, slot_mapping)
+    q_out = torch.empty(query.shape, dtype=dtype, device=dev)
+    k_out = torch.empty(key.shape, dtype=dtype, device=dev) if return_key else None
+    T = query.shape[0]
+    if T:
+        es = 2
+        positions = positions.contiguous()
+        if kv_cache is not None:
+            NB, _, BS, H, D = kv_cache.shape
+            kptr = kv_cache.data_ptr()
+            cache = (kptr, kptr + BS * H * D * es, kv_cache.stride(0) * es, H * D * es, slots.data_ptr())
+            v_ptr, v_tok, bound = value.data_ptr(), value.stride(0) * es, NB * BS
+        else:
+            cache, v_ptr, v_tok, bound, BS = (None, None, 0, 0, None), None, 0, 0, 0
+        with _OnDevice(dev):
+            rc = _lib.lib().lms_qk_norm_rope_and_cache(
+                query.data_ptr(), key.data_ptr(), v_ptr, query.stride(0) * es, key.stride(0) * es, v_tok,
+                query_weight.data_ptr(), key_weight.data_ptr(), eps, positions.data_ptr(),
+                1 if positions.dtype == torch.int64 else 0, cos_sin_cache.data_ptr(),
+                cos_sin_cache.stride(0) * es, q_out.data_ptr(), q_out.stride(0) * es,
+                k_out.data_ptr() if return_key else None, k_out.stride(0) * es if return_key else 0,
+                *cache, T, query.shape[1] // head_dim, key.shape[1] // head_dim, head_dim,
+                _DTYPE_CODE[dtype], BS, bound, cos_sin_cache.shape[0], _stream_ptr(dev))
+        if rc:
+            _lib.check(rc)
+    return (q_out, k_out) if return_key else q_out
+
+
+def qk_norm_rotary_pos_emb(query: torch.Tensor, key: torch.Tensor, query_weight: torch.Tensor,
+                           key_weight: torch.Tensor, positions: torch.Tensor,
+                           cos_sin_cache: torch.Tensor, head_dim: int,
+                           eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(q_out, k_out)``: every head of ``query`` and ``key`` divided by its root mean square,
+    multiplied by ``query_weight`` / ``key_weight`` (``[head_dim]``, shared by the heads), and rotated
+    as :func:`rotary_pos_emb` does: ``x -> rotate(weight * x / sqrt(mean(x ** 2) + eps))``.
+
+    Evaluated in fp32 and rounded once.  Arguments and layouts are those of
+    :func:`rotary_pos_emb`; head dims are multiples of 16 up to 512.  A token whose position is
+    outside ``cos_sin_cache`` is not written (and reported by the debug checks)."""
+    return _qk_norm(query, key, None, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps,
+                    None, None, True)
+
+
+def qk_norm_rotary_pos_emb_and_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                                     query_weight: torch.Tensor, key_weight: torch.Tensor,
+                                     positions: torch.Tensor, cos_sin_cache: torch.Tensor, head_dim: int,
+                                     kv_cache: torch.Tensor, slot_mapping: torch.Tensor,
+                                     eps: float = 1e-6, return_key: bool = False):
+    """:func:`qk_norm_rotary_pos_emb` with the cache write of :func:`rotary_pos_emb_and_cache` in
+    the same launch: rotated K and ``value`` go to ``kv_cache`` (one layer, ``[num_blocks, 2,
+    block_size, H, D]``) at ``slot_mapping``, the rotated query is returned, with
+    ``return_key=True`` the rotated key too.  ``slot_mapping[t] < 0`` skips the cache write of token
+    ``t``; so does a slot beyond the cache (reported by the debug checks).  Slots must be distinct."""
+    return _qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps,
+                    kv_cache, slot_mapping, return_key)
