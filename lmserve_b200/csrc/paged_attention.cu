@@ -7,6 +7,7 @@
 //   s_j = scale * q_r . k_j,  m = max s_j,  l = sum exp(s_j - m),  out_r = sum exp(s_j - m) v_j / l
 //   lse_r = m + log l;  a row without any key: out = 0, lse = -inf.
 // Scores, m, l and the accumulator are fp32; out is rounded once.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -62,9 +63,76 @@ __device__ __forceinline__ long long key_offset(const AttentionParams& p, const 
   return (long long)page * p.block_stride + (long long)(key - pg * p.block_size) * p.slot_stride;
 }
 
-// One warp a row; a lane owns the element pairs lane, lane + 32, ... of the head.
-constexpr int kMaxPairs = 4;
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
+// One warp, one row: a lane owns the element pairs lane, lane + 32, ... of the head, up to PAIRS of
+// them.  Scores in base 2.  Keys that are not walked are not touched.
+template <bool BF16, int PAIRS>
+struct RowWalk {
+  float2 q[PAIRS], acc[PAIRS];
+  float m = -INFINITY, l = 0.f;
+
+  __device__ __forceinline__ RowWalk(const char* row, int head_dim, int lane) {
+#pragma unroll
+    for (int e = 0; e < PAIRS; ++e) {
+      const int at = lane + 32 * e;
+      q[e] = at < head_dim / 2 ? up2<BF16>(reinterpret_cast<const uint32_t*>(row)[at]) : make_float2(0.f, 0.f);
+      acc[e] = make_float2(0.f, 0.f);
+    }
+  }
+  __device__ __forceinline__ void walk(const AttentionParams& p, const PageList& list, int first_page, int kvh,
+                                       int key, int end, int lane) {
+    const int head = kvh * p.head_dim * 2;
+    for (; key < end; ++key) {
+      const long long off = key_offset(p, list, first_page, key);
+      const uint32_t* kp = reinterpret_cast<const uint32_t*>(p.kcache + off + head);
+      const uint32_t* vp = reinterpret_cast<const uint32_t*>(p.vcache + off + head);
+      float s = 0.f;
+      float2 v[PAIRS];
+#pragma unroll
+      for (int e = 0; e < PAIRS; ++e) {
+        const int at = lane + 32 * e;
+        float2 k = make_float2(0.f, 0.f);
+        v[e] = k;
+        if (at < p.head_dim / 2 && off >= 0) {
+          k = up2<BF16>(kp[at]);
+          v[e] = up2<BF16>(vp[at]);
+        }
+        s = fmaf(q[e].x, k.x, fmaf(q[e].y, k.y, s));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      s *= p.scale * kLog2e;
+      const float top = fmaxf(m, s);
+      const float keep = m == -INFINITY ? 0.f : exp2_fast(m - top);
+      const float w = s == -INFINITY ? 0.f : exp2_fast(s - top);
+      m = top;
+      l = l * keep + w;
+#pragma unroll
+      for (int e = 0; e < PAIRS; ++e) {
+        acc[e].x = fmaf(w, v[e].x, acc[e].x * keep);
+        acc[e].y = fmaf(w, v[e].y, acc[e].y * keep);
+      }
+    }
+  }
+  __device__ __forceinline__ float inverse() const { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }  // NaN stays
+  __device__ __forceinline__ float lse2() const { return l == 0.f ? -INFINITY : m + log2f(l); }
+  __device__ __forceinline__ void store(char* out, int head_dim, int lane) const {
+    const float inv = inverse();
+#pragma unroll
+    for (int e = 0; e < PAIRS; ++e)
+      if (lane + 32 * e < head_dim / 2)
+        reinterpret_cast<uint32_t*>(out)[lane + 32 * e] = down2<BF16>(acc[e].x * inv, acc[e].y * inv);
+  }
+};
+
+// Any head dim: one warp a row, on the CUDA cores.
 template <bool BF16>
 __global__ void __launch_bounds__(128) attention_rows_kernel(const AttentionParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -80,78 +148,20 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(const AttentionPara
     n_new = p.qo_indptr[b + 1] - p.qo_indptr[b];
     i = t - p.qo_indptr[b];
   }
-  const int pairs = p.head_dim / 2;
-  const int kv_head_bytes = (h / (p.num_heads / p.num_kv_heads)) * p.head_dim * 2;
-  const uint32_t* q = reinterpret_cast<const uint32_t*>(p.q + (long long)t * p.q_tok + (long long)h * p.head_dim * 2);
-  float2 qv[kMaxPairs], acc[kMaxPairs];
-#pragma unroll
-  for (int e = 0; e < kMaxPairs; ++e) {
-    const int at = lane + 32 * e;
-    qv[e] = at < pairs ? up2<BF16>(q[at]) : make_float2(0.f, 0.f);
-    acc[e] = make_float2(0.f, 0.f);
+  const int kvh = h / (p.num_heads / p.num_kv_heads);
+  RowWalk<BF16, 4> w(p.q + (long long)t * p.q_tok + (long long)h * p.head_dim * 2, p.head_dim, lane);
+  if (p.prefix.indptr != nullptr) {
+    const int g = p.group_indptr != nullptr ? last_not_above(p.group_indptr, p.num_groups + 1, b) : 0;
+    if (g >= 0 && g < p.num_groups)
+      w.walk(p, p.prefix, p.prefix.indptr[g], kvh, 0, list_keys(p.prefix, g, p.block_size), lane);
   }
-  float m = -INFINITY, l = 0.f;
-  for (int part = 0; part < 2; ++part) {
-    const PageList& list = part == 0 ? p.prefix : p.own;
-    if (list.indptr == nullptr) continue;
-    int which = b;
-    if (part == 0) {
-      which = p.group_indptr != nullptr ? last_not_above(p.group_indptr, p.num_groups + 1, b) : 0;
-      if (which < 0 || which >= p.num_groups) continue;
-    }
-    const int len = list_keys(list, which, p.block_size);
-    const int end = part == 1 && p.causal ? min(len, len - n_new + i + 1) : len;
-    const int first = list.indptr[which];
-    for (int key = 0; key < end; ++key) {
-      const long long off = key_offset(p, list, first, key);
-      const uint32_t* kp = reinterpret_cast<const uint32_t*>(p.kcache + off + kv_head_bytes);
-      const uint32_t* vp = reinterpret_cast<const uint32_t*>(p.vcache + off + kv_head_bytes);
-      float s = 0.f;
-      float2 v[kMaxPairs];
-#pragma unroll
-      for (int e = 0; e < kMaxPairs; ++e) {
-        const int at = lane + 32 * e;
-        float2 k = make_float2(0.f, 0.f);
-        v[e] = k;
-        if (at < pairs && off >= 0) {
-          k = up2<BF16>(kp[at]);
-          v[e] = up2<BF16>(vp[at]);
-        }
-        s = fmaf(qv[e].x, k.x, fmaf(qv[e].y, k.y, s));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      s *= p.scale;
-      const float top = fmaxf(m, s);
-      const float keep = m == -INFINITY ? 0.f : __expf(m - top);
-      const float w = s == -INFINITY ? 0.f : __expf(s - top);
-      m = top;
-      l = l * keep + w;
-#pragma unroll
-      for (int e = 0; e < kMaxPairs; ++e) {
-        acc[e].x = fmaf(w, v[e].x, acc[e].x * keep);
-        acc[e].y = fmaf(w, v[e].y, acc[e].y * keep);
-      }
-    }
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  uint32_t* o = reinterpret_cast<uint32_t*>(p.out + (long long)t * p.o_tok + (long long)h * p.head_dim * 2);
-#pragma unroll
-  for (int e = 0; e < kMaxPairs; ++e)
-    if (lane + 32 * e < pairs) o[lane + 32 * e] = down2<BF16>(acc[e].x * inv, acc[e].y * inv);
-  if (p.lse != nullptr && lane == 0) p.lse[row] = l > 0.f ? m + __logf(l) : -INFINITY;
+  const int len = list_keys(p.own, b, p.block_size);
+  w.walk(p, p.own, p.own.indptr[b], kvh, 0, p.causal ? min(len, len - n_new + i + 1) : len, lane);
+  w.store(p.out + (long long)t * p.o_tok + (long long)h * p.head_dim * 2, p.head_dim, lane);
+  if (p.lse != nullptr && lane == 0) p.lse[row] = w.lse2() * kLn2;
 }
-
 
 // ---------------------------------------------------------------- shared pieces of the matrix kernels
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
 __device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem, bool valid) {
   const int bytes = valid ? 16 : 0;  // the rest of the 16 bytes is filled with zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(bytes) : "memory");
@@ -209,14 +219,15 @@ struct DecodeParams {
   int n_ranges;        // equal runs of the page axis
   int hb_shift;        // log2 of the heads a CTA works on
   int units_per_page;  // 16-key units of a page
-  int whole_slot;      // first slot of whole requests when a join follows for every row, else -1
+  long long slot0;     // first slot of the runs
+  bool join_all;       // whole requests too go to a slot (behind the runs' own): a prefix follows
 };
 
 struct TileMeta {
   int request;
   int keys;   // keys of the tile that exist
   int flags;  // 1: first tile of the request in this warp, 2: last
-  int slot;   // where the result goes: -1 = the output row
+  int slot;   // where the result goes: -1 = the output row (a slot is num_heads rows)
 };
 
 template <int D, int NST>
@@ -319,8 +330,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
       key_end = (int)k1;
       first_page = (int)first;
       const bool whole = s0 >= u_begin && s1 <= u_end;
-      slot = whole ? (p.whole_slot < 0 ? -1 : p.whole_slot + request)
-                   : 2 * (int)blockIdx.x + (s0 < u_begin ? 0 : 1);
+      slot = whole ? (p.join_all ? (int)p.slot0 + 2 * p.n_ranges + request : -1)
+                   : (int)p.slot0 + 2 * (int)blockIdx.x + (s0 < u_begin ? 0 : 1);
       fresh = true;
       return;
     }
@@ -561,12 +572,503 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
   cp_async_wait<0>();
 }
 
+// ---------------------------------------------------------------- tiles of rows
+// Many rows share their keys: the tokens of one request (or of all requests of a prefix group)
+// times the G heads of a key head.  Two row tiles of 128 (row = token * G + head) and one stream
+// of 128-key tiles per CTA; S = Q K^T and O += P V run on the tensor cores (tcgen05, M = 128) with
+// S, P and O in tensor memory.
+//
+//   warps 0-3, 4-7   softmax of row tile 0 / 1, one thread a row: S from tensor memory, running
+//                    maximum and sum, P = 2^(S - m) in the element type over S's own columns
+//   warp 8, 9        K / V tiles into two-or-more-stage rings
+//   warp 10          issues the MMAs: PV of a tile, then the next QK of the same row tile, so that
+//                    one row tile's softmax runs beside the other's products
+//
+// The maximum is only moved (and O rescaled in tensor memory, by the softmax threads) when it
+// grows by more than 2^8: P and l may exceed 1 by that factor, which fp32 sums and 16-bit P hold.
+// S of the next tile overwrites P: it is issued behind the PV that reads it, and the commit behind
+// it tells the softmax warps that this PV, too, is complete.  P is rounded to the element type
+// (half a step, 2^-8 in bf16): the tensor cores take no wider second operand.
+//
+// Pages of 8 to 128 keys (powers of two) and of multiples of 128 are loaded by TMA, one box a page
+// and 64-element half row, 128-byte swizzled; a tile that reaches past the last key, and other page
+// sizes, by cp.async rows with zeros behind the last key (what lies there may be anything, and 0 * NaN
+// is not 0).
+constexpr int kRows = 128;       // rows of a tile
+constexpr int kKeys = 128;       // keys of a tile
+constexpr int kTileThreads = 384;
+constexpr float kLazy = 8.f;     // log2 of the factor the maximum may lag behind
+
+struct TileParams {
+  CUtensorMap kmap, vmap;
+  AttentionParams a;
+  PageList list;      // pages of each sequence (a request's own, or a group's prefix)
+  Partials part;
+  int shared;         // 1: sequences are prefix groups, 0: requests
+  int n_seq, n_slots, n_splits;
+  int slot0;          // first of n_splits sets of partials ([num_tokens] slots each), -1: final
+  int causal;
+  int box;            // keys of a TMA box, 0 = no TMA
+};
+
+template <int D>
+struct TileSmem {
+  static constexpr int kStages = D == 64 ? 4 : 2;
+  static constexpr int kStage = kKeys * D * 2;
+  static constexpr int kV = 0, kK = kStages * kStage, kQ = 2 * kStages * kStage;
+  static constexpr int kBytes = kQ + 2 * kRows * D * 2;
+};
+
+struct TileBars {
+  uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
+  uint64_t qfull, sfull[2], pfull[2], ofull[2], done;
+  uint32_t tmem;
+  int dead;
+};
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 consecutive columns of the thread's own tensor memory lane.
+__device__ __forceinline__ void tc_ld32(uint32_t* r, uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// Shared memory operand: rows (or K groups) of 128 bytes, 128-byte swizzle, 8-row groups 1024 bytes
+// apart; lbo: bytes between 64-element chunks of an operand whose rows run along K.
+__device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t lbo) {
+  return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// kind::f16, fp32 accumulators: element type (0 fp16, 1 bf16), M = 128, N, B along K or along N.
+__device__ __forceinline__ constexpr uint32_t umma_idesc(bool bf16, int n, bool b_along_n) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_along_n ? 1u : 0u) << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+      "r"(add ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+      "r"(add ? 1u : 0u)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// First token of sequence i (i <= n_seq).
+__device__ __forceinline__ int token_of(const TileParams& p, int i) {
+  if (p.shared) i = p.a.group_indptr != nullptr ? min(max(p.a.group_indptr[i], 0), p.a.num_requests)
+                                                : (i > 0 ? p.a.num_requests : 0);
+  return p.a.qo_indptr != nullptr ? p.a.qo_indptr[i] : i;
+}
+
+// Loads 128 keys of one plane into a stage.  One warp.
+template <int D>
+__device__ __forceinline__ void load_tile(const TileParams& p, const CUtensorMap* map, const char* cache, int kvh,
+                                          int first_page, int len, int tile, uint32_t dst, uint64_t* full, int lane) {
+  const AttentionParams& a = p.a;
+  constexpr int kHalves = D / 64, kHalf = kKeys * 128;
+  const int key0 = tile * kKeys;
+  if (p.box > 0 && key0 + kKeys <= len) {
+    if (lane == 0) mbar_expect_tx(full, kKeys * D * 2);
+    __syncwarp();
+    const int pieces = kKeys / p.box * kHalves;
+    if (lane < pieces) {
+      const int piece = lane / kHalves, half = lane - piece * kHalves;
+      const int key = key0 + piece * p.box;
+      const int pg = key / a.block_size;
+      const long long at = (long long)first_page + pg;
+      int page = -1;  // outside the map: the box is filled with zeros
+      if (at >= 0 && at < p.list.num_indices) {
+        page = p.list.indices[at];
+        if (page < 0 || page >= a.num_blocks) {
+          if (a.checks) report(a.err, kErrBadPage, kWhereAttention, at, page);
+          page = -1;
+        }
+      }
+      tma_load4(dst + half * kHalf + piece * p.box * 128, map, full, half * 64, key - pg * a.block_size, kvh, page);
+    }
+    return;
+  }
+  const char* head = cache + (long long)kvh * D * 2;
+  constexpr int kChunks = D / 8, kRowsAtOnce = 32 / kChunks;
+#pragma unroll 1
+  for (int base = 0; base < kKeys; base += 32) {
+    long long off = -1;
+    const int key = key0 + base + lane;
+    if (key < len) off = key_offset(a, p.list, first_page, key);
+#pragma unroll 4
+    for (int i = 0; i < 32 / kRowsAtOnce; ++i) {
+      const int src = i * kRowsAtOnce + lane / kChunks, row = base + src, c = lane % kChunks;
+      const long long o = __shfl_sync(0xffffffffu, off, src);
+      cp_async16(dst + (c >> 3) * kHalf + row * 128 + (((c & 7) ^ (row & 7)) << 4), o >= 0 ? head + o + c * 16 : cache, o >= 0);
+    }
+  }
+  cp_async_commit();
+  cp_async_wait<0>();
+  fence_proxy_async();  // generic-proxy writes, read by the tensor cores
+  __syncwarp();
+  if (lane == 0) mbar_arrive(full);
+}
+
+template <bool BF16, int D>
+__global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const __grid_constant__ TileParams p) {
+  using S = TileSmem<D>;
+  constexpr int ST = S::kStages, kHalf = kKeys * 128;
+  extern __shared__ __align__(1024) char smem_raw[];
+  __shared__ TileBars bars;
+  const AttentionParams& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.num_heads / a.num_kv_heads;
+  const int kvh = blockIdx.y;
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // The sequence of this slot: sequence i has the slots from rows(i) / 256 + i on, which leaves it
+  // enough of them without a scan; some stay empty.  Late slots, with the longest causal rows, first.
+  const int slot = p.n_slots - 1 - (int)blockIdx.x;
+  const int token0 = token_of(p, 0);
+  int seq = 0;
+  {
+    int lo = 0, n = p.n_seq;
+    while (n > 1) {
+      const int step = (n + 31) / 32, at = lo + lane * step;
+      const bool below = lane * step < n && (long long)(token_of(p, at) - token0) * G / (2 * kRows) + at <= slot;
+      const int last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
+      n = min(step, n - last * step);
+      lo += last * step;
+    }
+    seq = lo;
+  }
+  const int t_begin = token_of(p, seq), t_end = min(token_of(p, seq + 1), a.num_tokens);
+  const int n_new = t_end - t_begin;
+  const long long first_slot = (long long)(t_begin - token0) * G / (2 * kRows) + seq;
+  const long long row0 = (slot - first_slot) * (2 * kRows);
+  const long long n_rows = (long long)n_new * G;
+  if (t_begin < 0 || row0 < 0 || row0 >= n_rows) return;
+  const int rows = (int)min(n_rows - row0, 2ll * kRows);
+  const int n_tiles = rows > kRows ? 2 : 1;
+
+  // keys: to the last one that the last row reads
+  const int len = list_keys(p.list, seq, a.block_size);
+  int k_end = len;
+  if (p.causal) k_end = min(len, max(0, len - n_new + (int)((row0 + rows - 1) / G) + 1));
+  const int kv_tiles = (k_end + kKeys - 1) / kKeys;
+  const int tile0 = (int)((long long)kv_tiles * blockIdx.z / p.n_splits);
+  const int n_kv = (int)((long long)kv_tiles * (blockIdx.z + 1) / p.n_splits) - tile0;
+
+  // this thread's row (softmax warps)
+  const int r = threadIdx.x;                       // row of the tile pair
+  const bool has_row = r < rows && r < 2 * kRows;
+  const int tok = (int)((row0 + r) / G), g = (int)((row0 + r) - (long long)tok * G);
+  const long long out_row = (long long)(t_begin + tok) * a.num_heads + kvh * G + g;  // [token][head]
+  const long long part_row = ((long long)(p.slot0 + (int)blockIdx.z) * a.num_tokens) * a.num_heads + out_row;
+
+  if (n_kv <= 0) {  // nothing to read: an empty part, or rows of zeros
+    if (has_row) {
+      if (p.slot0 >= 0) {
+        p.part.lse[part_row] = -INFINITY;
+      } else {
+        char* o = a.out + (long long)(t_begin + tok) * a.o_tok + (long long)(kvh * G + g) * D * 2;
+        for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(o + i * 16) = make_uint4(0, 0, 0, 0);
+        if (a.lse != nullptr) a.lse[out_row] = -INFINITY;
+      }
+    }
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&bars.kfull[s], 1);
+      mbar_init(&bars.kempty[s], 1);
+      mbar_init(&bars.vfull[s], 1);
+      mbar_init(&bars.vempty[s], 1);
+    }
+    mbar_init(&bars.qfull, 2 * kRows);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.sfull[i], 1);
+      mbar_init(&bars.pfull[i], kRows);
+      mbar_init(&bars.ofull[i], 1);
+    }
+    mbar_init(&bars.done, 1);
+    bars.dead = 0;
+    mbar_fence_init();
+  }
+  if (warp == 10) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&bars.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  const uint32_t sm_q = smem + S::kQ, sm_k = smem + S::kK, sm_v = smem + S::kV;
+  const int first_page = p.list.indptr[seq];
+  const float scale2 = fabsf(a.scale) * kLog2e;
+
+  // A wait that runs out ends the role; the others run out in turn, and the CTA leaves in order.
+  auto wait = [&](uint64_t* bar, unsigned parity) -> bool {
+    const bool ok = mbar_wait_bounded(bar, parity);
+    if (!ok) report(a.err, kErrWaitTimeout, kWhereAttention, blockIdx.x, bar - bars.kfull);
+    return __all_sync(0xffffffffu, ok);  // a warp goes on or leaves as one
+  };
+
+  if (warp < 8) {
+    // ------------------------------------------------ softmax
+    const int i = warp >> 2;
+    {  // Q row -> shared memory; rows that do not exist are zeros
+      const char* src = a.q + (long long)(t_begin + tok) * a.q_tok + (long long)(kvh * G + g) * D * 2;
+      const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+      const int row = r & (kRows - 1);
+      const uint32_t dst = sm_q + i * kRows * D * 2 + row * 128;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (has_row) v = *reinterpret_cast<const uint4*>(src + c * 16);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * (kRows * 128) + (((c & 7) ^ (row & 7)) << 4)),
+                     "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip) : "memory");
+      }
+      fence_proxy_async();
+      mbar_arrive(&bars.qfull);
+    }
+    if (i < n_tiles) {
+      const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // lane 32 * (warp % 4) in bits 16..
+      const uint32_t t_s = lanes + i * 128, t_o = lanes + 256 + i * 128;
+      const bool live = (r & ~31) < rows;  // the warp has a row
+      const int limit = p.causal ? min(len, len - n_new + tok + 1) : len;  // keys below it are read
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < n_kv; ++j) {
+        if (!(ok = wait(&bars.sfull[i], j & 1))) break;
+        tc_fence_after();
+        if (live) {
+          float s[kKeys];
+          uint32_t* raw = reinterpret_cast<uint32_t*>(s);
+#pragma unroll
+          for (int c = 0; c < kKeys; c += 32) tc_ld32(raw + c, t_s + c);
+          tc_wait_ld();
+          const int seen = limit - (tile0 + j) * kKeys;
+          if (!__all_sync(0xffffffffu, seen >= kKeys)) {
+#pragma unroll
+            for (int c = 0; c < kKeys; ++c)
+              if (c >= seen) s[c] = -INFINITY;
+          }
+          float top = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < kKeys; ++c) top = fmaxf(top, s[c]);
+          top = top == -INFINITY ? top : top * scale2;
+          float keep = 1.f;
+          if (top > m + kLazy) {
+            keep = exp2_fast(m - top);
+            m = top;
+          }
+          const bool moved = __any_sync(0xffffffffu, keep != 1.f);
+          const float base = m == -INFINITY ? 0.f : m;
+          float sum = 0.f;
+          uint32_t w[kKeys / 2];
+#pragma unroll
+          for (int c = 0; c < kKeys; c += 2) {
+            const float x = exp2_fast(fmaf(s[c], scale2, -base)), y = exp2_fast(fmaf(s[c + 1], scale2, -base));
+            sum += x + y;
+            w[c / 2] = down2<BF16>(x, y);
+          }
+          l = fmaf(l, keep, sum);
+          tc_st32(t_s, w);
+          tc_st32(t_s + 32, w + 32);
+          if (moved && j > 0) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tc_ld32(o, t_o + c);
+              tc_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+              tc_st32(t_o + c, o);
+            }
+          }
+          tc_wait_st();
+        }
+        tc_fence_before();
+        mbar_arrive(&bars.pfull[i]);
+      }
+      if (ok && wait(&bars.ofull[i], 0) && live) {
+        tc_fence_after();
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays
+        char* const dst = a.out + (long long)(t_begin + tok) * a.o_tok + (long long)(kvh * G + g) * D * 2;
+        float finite = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tc_ld32(o, t_o + c);
+          tc_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) finite = fmaf(__uint_as_float(o[e]), 0.f, finite);
+          if (!has_row) {
+          } else if (p.slot0 >= 0) {
+            float4* d = reinterpret_cast<float4*>(p.part.out + part_row * D + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              d[e] = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
+                                 __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
+          } else {
+            uint4* d = reinterpret_cast<uint4*>(dst + c * 2);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t v[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                v[x] = down2<BF16>(__uint_as_float(o[8 * e + 2 * x]) * inv, __uint_as_float(o[8 * e + 2 * x + 1]) * inv);
+              d[e] = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          }
+          __syncwarp();
+        }
+        if (has_row) {
+          const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
+          if (p.slot0 >= 0) p.part.lse[part_row] = lse2;
+          else if (a.lse != nullptr) a.lse[out_row] = lse2 * kLn2;
+        }
+        // A key masked for this row but not for the whole tile took part in PV with weight 0, and
+        // 0 * infinity is NaN: a causal row that is not finite is done again by itself.
+        __syncwarp();
+        unsigned again = __ballot_sync(0xffffffffu, p.causal && has_row && finite != 0.f);
+        while (again != 0) {
+          const int who = __ffs(again) - 1;
+          again &= again - 1;
+          const int w_tok = __shfl_sync(0xffffffffu, tok, who), w_g = __shfl_sync(0xffffffffu, g, who);
+          const int w_end = min(__shfl_sync(0xffffffffu, limit, who), (tile0 + n_kv) * kKeys);
+          const long long w_part = __shfl_sync(0xffffffffu, part_row, who), w_out = __shfl_sync(0xffffffffu, out_row, who);
+          const long long head = (long long)(kvh * G + w_g) * D * 2;
+          RowWalk<BF16, D / 64> walk(a.q + (long long)(t_begin + w_tok) * a.q_tok + head, D, lane);
+          walk.walk(a, p.list, first_page, kvh, tile0 * kKeys, w_end, lane);
+          if (p.slot0 < 0) {
+            walk.store(a.out + (long long)(t_begin + w_tok) * a.o_tok + head, D, lane);
+            if (a.lse != nullptr && lane == 0) a.lse[w_out] = walk.lse2() * kLn2;
+          } else {
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e)
+              reinterpret_cast<float2*>(p.part.out + w_part * D)[lane + 32 * e] =
+                  make_float2(walk.acc[e].x * walk.inverse(), walk.acc[e].y * walk.inverse());
+            if (lane == 0) p.part.lse[w_part] = walk.lse2();
+          }
+        }
+        tc_fence_before();
+      }
+    }
+  } else if (warp < 10) {
+    // ------------------------------------------------ K (warp 8) and V (warp 9)
+    const bool is_k = warp == 8;
+    uint64_t* full = is_k ? bars.kfull : bars.vfull;
+    uint64_t* empty = is_k ? bars.kempty : bars.vempty;
+    int j = 0;
+    for (; j < n_kv; ++j) {
+      const int s = j % ST, use = j / ST;
+      if (use > 0 && !wait(&empty[s], (use - 1) & 1)) break;
+      load_tile<D>(p, is_k ? &p.kmap : &p.vmap, is_k ? a.kcache : a.vcache, kvh, first_page, len, tile0 + j,
+                   (is_k ? sm_k : sm_v) + s * S::kStage, &full[s], lane);
+    }
+    // no copy may be in flight when the CTA leaves, whatever the others did
+    for (int d = max(0, j - ST); d < j; ++d) wait(&full[d % ST], (d / ST) & 1);
+  } else if (warp == 10) {
+    // ------------------------------------------------ MMAs
+    constexpr uint32_t id_s = umma_idesc(BF16, kKeys, false), id_o = umma_idesc(BF16, D, true);
+    auto qk = [&](int i, int s) {
+      if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k >> 2) * (kRows * 128) + (k & 3) * 32;
+          umma_ss(tmem + i * 128, umma_desc(sm_q + i * kRows * D * 2 + off, 16), umma_desc(sm_k + s * S::kStage + off, 16), id_s, k > 0);
+        }
+        tc_commit(&bars.sfull[i]);
+      }
+      __syncwarp();
+    };
+    bool ok = wait(&bars.qfull, 0) && wait(&bars.kfull[0], 0);
+    if (ok) {
+      tc_fence_after();
+      for (int i = 0; i < n_tiles; ++i) qk(i, 0);
+      if (lane == 0) tc_commit(&bars.kempty[0]);
+      for (int j = 0; ok && j < n_kv; ++j) {
+        const int s = j % ST, n = (j + 1) % ST;
+        if (!(ok = wait(&bars.vfull[s], (j / ST) & 1))) break;
+        if (j + 1 < n_kv && !(ok = wait(&bars.kfull[n], ((j + 1) / ST) & 1))) break;
+        for (int i = 0; i < n_tiles; ++i) {
+          if (!(ok = wait(&bars.pfull[i], j & 1))) break;
+          tc_fence_after();
+          if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)
+              umma_ts(tmem + 256 + i * 128, tmem + i * 128 + k * 8, umma_desc(sm_v + s * S::kStage + k * 2048, kHalf), id_o, j > 0 || k > 0);
+            if (j + 1 == n_kv) tc_commit(&bars.ofull[i]);
+            if (i + 1 == n_tiles) tc_commit(&bars.vempty[s]);
+          }
+          __syncwarp();
+          if (j + 1 < n_kv) qk(i, n);
+        }
+        if (ok && j + 1 < n_kv && lane == 0) tc_commit(&bars.kempty[n]);
+      }
+    }
+    if (lane == 0) tc_commit(&bars.done);
+    __syncwarp();
+    wait(&bars.done, 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 10) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
 // ---------------------------------------------------------------- join
-// One warp a row: the row's partials, weighted by 2^(lse - max lse).  A row of a request that one
-// run held whole is finished already; a request without any key gets its zeros here.
+// One warp a row: the row's partials, weighted by 2^(lse - max lse).  Sets [0, n_shared) come from
+// the prefix, [n_shared, n_sets) from the own keys, one slot a token each; behind them the slots of
+// the decode kernel's runs.
 struct JoinParams {
   AttentionParams a;
   Partials part;
+  int n_shared, n_sets;
+  bool runs;        // the own keys were read by the decode kernel
+  bool all;         // its whole requests, too, lie in slots
   int n_ranges, units_per_page;
 };
 
@@ -579,52 +1081,86 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams p)
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int t = (int)(row / a.num_heads), h = (int)(row - (long long)t * a.num_heads);
   if (t >= a.num_tokens) return;
-  const int* indptr = a.own.indptr;
-  const long long axis0 = indptr[0];
-  const long long units = ((long long)indptr[a.num_requests] - axis0) * p.units_per_page;
-  const long long chunk = (units + p.n_ranges - 1) / p.n_ranges;
-  const long long s0 = (indptr[t] - axis0) * p.units_per_page, s1 = (indptr[t + 1] - axis0) * p.units_per_page;
-  int x0 = 0, x1 = -1;  // the runs that hold a part of the request
-  if (s1 > s0 && chunk > 0) {
-    x0 = (int)min(max(s0 / chunk, 0ll), p.n_ranges - 1ll);
-    x1 = (int)min(max((s1 - 1) / chunk, 0ll), p.n_ranges - 1ll);
-    if (x0 == x1) return;
-  }
   constexpr int E = D / 32;
   float acc[E] = {}, m = -INFINITY, l = 0.f;
-  for (int x = x0; x <= x1; ++x) {
-    const long long at = (long long)(2 * x + (x == x0 ? 1 : 0)) * a.num_heads + h;
+  auto add = [&](long long slot) {
+    const long long at = slot * a.num_heads + h;
     const float s = p.part.lse[at];
-    if (s == -INFINITY) continue;
+    if (s == -INFINITY) return;
     const float top = fmaxf(m, s), keep = exp2_fast(m - top), w = exp2_fast(s - top);
     m = top;
     l = l * keep + w;
     const float* v = p.part.out + at * D + lane * E;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[e], acc[e] * keep);
+  };
+  int first = 0;
+  if (a.qo_indptr != nullptr && (t < a.qo_indptr[0] || t >= a.qo_indptr[a.num_requests])) return;  // left as it is
+  if (p.n_shared > 0 && a.group_indptr != nullptr) {
+    // a request outside every group has no set from the prefix
+    const int b0 = min(max(a.group_indptr[0], 0), a.num_requests);
+    const int b1 = min(max(a.group_indptr[a.num_groups], 0), a.num_requests);
+    const int t0 = a.qo_indptr != nullptr ? a.qo_indptr[b0] : b0, t1 = a.qo_indptr != nullptr ? a.qo_indptr[b1] : b1;
+    if (t < t0 || t >= t1) first = p.n_shared;
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  if (p.runs) {
+    const int* indptr = a.own.indptr;
+    const long long axis0 = indptr[0];
+    const long long units = ((long long)indptr[a.num_requests] - axis0) * p.units_per_page;
+    const long long chunk = (units + p.n_ranges - 1) / p.n_ranges;
+    const long long s0 = (indptr[t] - axis0) * p.units_per_page, s1 = (indptr[t + 1] - axis0) * p.units_per_page;
+    const long long slot0 = (long long)p.n_sets * a.num_tokens;
+    if (s1 > s0 && chunk > 0) {  // the runs that hold a part of the request
+      const int x0 = (int)min(max(s0 / chunk, 0ll), p.n_ranges - 1ll);
+      const int x1 = (int)min(max((s1 - 1) / chunk, 0ll), p.n_ranges - 1ll);
+      if (x0 == x1) {
+        if (!p.all) return;  // finished by its run
+        add(slot0 + 2 * p.n_ranges + t);
+      } else {
+        for (int x = x0; x <= x1; ++x) add(slot0 + 2 * x + (x == x0 ? 1 : 0));
+      }
+    }
+  }
+  for (int x = first; x < p.n_sets; ++x) add((long long)x * a.num_tokens + t);
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   uint32_t* out = reinterpret_cast<uint32_t*>(a.out + (long long)t * a.o_tok + ((long long)h * D + lane * E) * 2);
 #pragma unroll
   for (int e = 0; e < E; e += 2) out[e / 2] = down2<BF16>(acc[e] * inv, acc[e + 1] * inv);
-  if (a.lse != nullptr && lane == 0) a.lse[row] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  if (a.lse != nullptr && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // ---------------------------------------------------------------- launch rules
 // What a call launches, from its counts alone.
 struct Plan {
-  bool decode;         // one token a request, no shared prefix
+  bool rows;                 // the kernel for any head dim does it all
+  bool runs;                 // own keys by the decode kernel
   int n_ranges, hb_shift, units_per_page;
-  long long slots;     // partials
+  int shared_splits, own_splits;  // key splits of the tile kernel: prefix, own keys (0 = not launched)
+  bool join;
+  long long slots;           // of partials, num_heads rows each
 };
+
+// Splits of the keys so that the row tiles fill the GPU, 512 keys a split at least.
+int splits_of(long long tokens, long long seqs, long long pages, const AttentionParams& p, int sms) {
+  const int G = p.num_heads / p.num_kv_heads;
+  long long tiles = (tokens * G + 2 * kRows - 1) / (2 * kRows);
+  if (tiles < seqs) tiles = seqs;
+  const long long keys = pages * p.block_size / (seqs > 0 ? seqs : 1);
+  long long n = sms / (tiles * p.num_kv_heads);
+  if (n > keys / 512) n = keys / 512;
+  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
 
 Plan plan_of(const AttentionParams& p, int sms) {
   Plan r{};
   const int G = p.num_heads / p.num_kv_heads;
+  const bool shared = p.prefix.indptr != nullptr;
   r.units_per_page = (p.block_size + kTile - 1) / kTile;
-  r.decode = p.qo_indptr == nullptr && p.own.indptr != nullptr && p.prefix.indptr == nullptr && G <= 16 &&
-             (p.head_dim == 64 || p.head_dim == 128);
-  if (r.decode) {
+  r.rows = p.head_dim != 64 && p.head_dim != 128;
+  if (r.rows) return r;
+  r.runs = p.qo_indptr == nullptr && G <= 16;
+  if (shared) r.shared_splits = splits_of(p.num_tokens, p.num_groups, p.prefix.num_indices, p, sms);
+  if (r.runs) {
     // One CTA an SM.  The more heads a CTA takes, the fewer warps meet when a request ends, but
     // the shorter the runs: a run should hold 16 units at least for each request that it cuts.
     const long long units = (p.own.num_indices + 1) * r.units_per_page;
@@ -635,8 +1171,13 @@ Plan plan_of(const AttentionParams& p, int sms) {
     r.hb_shift = shift;
     r.n_ranges = sms / blocks(shift);
     if (r.n_ranges < 1) r.n_ranges = 1;
-    r.slots = 2ll * r.n_ranges;
+    r.slots = 2ll * r.n_ranges + (shared ? p.num_requests : 0);
+    r.join = true;
+  } else {
+    r.own_splits = splits_of(p.num_tokens, p.num_requests, p.own.num_indices, p, sms);
+    r.join = shared || r.own_splits > 1;
   }
+  if (r.join) r.slots += (long long)(r.shared_splits + r.own_splits) * p.num_tokens;
   return r;
 }
 
@@ -665,52 +1206,137 @@ struct Launch {
 };
 
 template <bool BF16, int D, int NST>
-cudaError_t launch_decode(const AttentionParams& p, const Plan& plan, bool pdl, int* launches, cudaStream_t stream) {
+cudaError_t launch_decode(const AttentionParams& p, const Plan& plan, bool pdl, cudaStream_t stream) {
   DecodeParams d{};
   d.a = p;
   d.part = partials_at(p, plan);
   d.n_ranges = plan.n_ranges;
   d.hb_shift = plan.hb_shift;
   d.units_per_page = plan.units_per_page;
-  d.whole_slot = -1;
+  d.slot0 = (long long)(plan.shared_splits + plan.own_splits) * p.num_tokens;
+  d.join_all = plan.shared_splits > 0;
   const int G = p.num_heads / p.num_kv_heads, HB = 1 << plan.hb_shift;
   auto kernel = attention_decode_kernel<BF16, D, NST>;
   const int smem = DecodeSmem<D, NST>::bytes(G, HB);
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   Launch go(dim3(plan.n_ranges, (p.num_kv_heads + HB - 1) / HB), kDecodeWarps * 32, smem, pdl, stream);
-  e = cudaLaunchKernelEx(&go.cfg, kernel, d);
+  return cudaLaunchKernelEx(&go.cfg, kernel, d);
+}
+
+// The driver's encoder, through the runtime (the library links no libcuda).
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encoder() {
+  static const EncodeTiled fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    cudaGetLastError();
+    return reinterpret_cast<EncodeTiled>(f);
+  }();
+  return fn;
+}
+
+// [page][head][entry][element] of one plane; false where TMA cannot address it.
+bool encode_plane(const AttentionParams& p, const char* base, int box, CUtensorMap* map) {
+  const EncodeTiled fn = encoder();
+  if (fn == nullptr || p.num_blocks < 1) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.block_size, (cuuint64_t)p.num_kv_heads, (cuuint64_t)p.num_blocks};
+  const cuuint64_t strides[3] = {(cuuint64_t)p.slot_stride, (cuuint64_t)p.head_dim * 2, (cuuint64_t)p.block_stride};
+  const cuuint32_t box_dims[4] = {64, (cuuint32_t)box, 1, 1}, ones[4] = {1, 1, 1, 1};
+  return fn(map, p.is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<char*>(base),
+            dims, strides, box_dims, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool BF16, int D>
+cudaError_t launch_tile(const AttentionParams& p, const Plan& plan, bool shared, bool pdl, cudaStream_t stream) {
+  TileParams t{};
+  t.a = p;
+  t.list = shared ? p.prefix : p.own;
+  t.part = partials_at(p, plan);
+  t.shared = shared;
+  t.n_seq = shared ? p.num_groups : p.num_requests;
+  const int G = p.num_heads / p.num_kv_heads;
+  const long long slots = (long long)p.num_tokens * G / (2 * kRows) + t.n_seq;
+  t.n_splits = shared ? plan.shared_splits : plan.own_splits;
+  if (slots > 0x7fffffffll || p.num_kv_heads > 65535) return cudaErrorInvalidConfiguration;
+  t.n_slots = (int)slots;
+  t.slot0 = plan.join ? (shared ? 0 : plan.shared_splits) : -1;
+  t.causal = !shared && p.causal;
+  const int bs = p.block_size;
+  if (bs % kKeys == 0) t.box = kKeys;
+  else if (bs >= 8 && bs < kKeys && kKeys % bs == 0) t.box = bs;
+  if (t.box > 0 && !(encode_plane(p, p.kcache, t.box, &t.kmap) && encode_plane(p, p.vcache, t.box, &t.vmap))) t.box = 0;
+  auto kernel = attention_tile_kernel<BF16, D>;
+  const int smem = TileSmem<D>::kBytes + 1024;  // rounded up to the swizzle's 1024-byte pattern
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
+  Launch go(dim3(t.n_slots, p.num_kv_heads, t.n_splits), kTileThreads, smem, pdl, stream);
+  return cudaLaunchKernelEx(&go.cfg, kernel, t);
+}
+
+template <bool BF16, int D>
+cudaError_t launch_join(const AttentionParams& p, const Plan& plan, bool pdl, cudaStream_t stream) {
   JoinParams j{};
   j.a = p;
-  j.part = d.part;
+  j.part = partials_at(p, plan);
+  j.n_shared = plan.shared_splits;
+  j.n_sets = plan.shared_splits + plan.own_splits;
+  j.runs = plan.runs;
+  j.all = plan.shared_splits > 0;
   j.n_ranges = plan.n_ranges;
   j.units_per_page = plan.units_per_page;
   const long long ctas = ((long long)p.num_tokens * p.num_heads + 3) / 4;
   if (ctas > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  Launch join(dim3((unsigned)ctas), 128, 0, pdl, stream);
-  *launches = 2;
-  return cudaLaunchKernelEx(&join.cfg, attention_join_kernel<BF16, D>, j);
+  Launch go(dim3((unsigned)ctas), 128, 0, pdl, stream);
+  return cudaLaunchKernelEx(&go.cfg, attention_join_kernel<BF16, D>, j);
 }
 
 template <bool BF16>
-cudaError_t launch_rows(const AttentionParams& p, bool pdl, int* launches, cudaStream_t stream) {
+cudaError_t launch_rows(const AttentionParams& p, bool pdl, cudaStream_t stream) {
   const long long ctas = ((long long)p.num_tokens * p.num_heads + 3) / 4;
   if (ctas > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   Launch go(dim3((unsigned)ctas), 128, 0, pdl, stream);
-  *launches = 1;
   return cudaLaunchKernelEx(&go.cfg, attention_rows_kernel<BF16>, p);
+}
+
+template <bool BF16, int D>
+cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, bool pdl, int* launches, cudaStream_t stream) {
+  cudaError_t e = cudaSuccess;
+  if (plan.shared_splits > 0) {
+    e = launch_tile<BF16, D>(p, plan, true, pdl, stream);
+    *launches += e == cudaSuccess;
+  }
+  if (e == cudaSuccess && plan.runs) {
+    const bool few = p.num_heads / p.num_kv_heads <= 8;
+    e = D == 64 ? launch_decode<BF16, 64, 5>(p, plan, pdl, stream)
+        : few   ? launch_decode<BF16, 128, 3>(p, plan, pdl, stream)
+                : launch_decode<BF16, 128, 2>(p, plan, pdl, stream);
+    *launches += e == cudaSuccess;
+  } else if (e == cudaSuccess) {
+    e = launch_tile<BF16, D>(p, plan, false, pdl, stream);
+    *launches += e == cudaSuccess;
+  }
+  if (e == cudaSuccess && plan.join) {
+    e = launch_join<BF16, D>(p, plan, pdl, stream);
+    *launches += e == cudaSuccess;
+  }
+  return e;
 }
 
 template <bool BF16>
 cudaError_t launch_typed(const AttentionParams& p, const Plan& plan, bool pdl, int* launches, cudaStream_t stream) {
-  if (plan.decode) {
-    const bool few = p.num_heads / p.num_kv_heads <= 8;
-    if (p.head_dim == 64) return launch_decode<BF16, 64, 5>(p, plan, pdl, launches, stream);
-    return few ? launch_decode<BF16, 128, 3>(p, plan, pdl, launches, stream)
-               : launch_decode<BF16, 128, 2>(p, plan, pdl, launches, stream);
+  if (plan.rows) {
+    *launches = 1;
+    return launch_rows<BF16>(p, pdl, stream);
   }
-  return launch_rows<BF16>(p, pdl, launches, stream);
+  return p.head_dim == 64 ? launch_matrix<BF16, 64>(p, plan, pdl, launches, stream)
+                          : launch_matrix<BF16, 128>(p, plan, pdl, launches, stream);
 }
 
 }  // namespace
@@ -723,6 +1349,7 @@ long long attention_workspace_bytes(const AttentionParams& p, int sms) {
 
 cudaError_t launch_attention(const AttentionParams& p, int sms, bool pdl, int* launches, cudaStream_t stream) {
   const Plan plan = plan_of(p, sms);
+  *launches = 0;
   return p.is_bf16 ? launch_typed<true>(p, plan, pdl, launches, stream)
                    : launch_typed<false>(p, plan, pdl, launches, stream);
 }
