@@ -191,6 +191,18 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+constexpr float kLazy = 8.f;     // log2 of the factor a running maximum may lag behind
+
 // A part of a row's softmax that another launch joins: out / l and lse in base 2.
 struct Partials {
   float* lse;  // [slots][num_heads]
@@ -206,99 +218,115 @@ struct Partials {
 // earlier run, else 2x + 1) for the join kernel.
 //
 // Inside a CTA a warp works alone: head hs = w % HB of the block, every KS-th 16-key tile of the
-// run (KS = 8 / HB), its own ring of cp.async stages, no block-wide barrier in the loop.  Q (16
-// rows, G of them used) stays in registers as the A operand of m16n8k16; K and V tiles are read
-// with ldmatrix from rows swizzled by 16-byte chunk ^ (row & 7).  The KS warps of a head join
-// their (m, l, out) through shared memory when a request ends.
+// run (KS = 8 / HB), its own ring of stages filled by TMA (a box a page, 128-byte swizzled) or, for
+// page sizes a 16-key box does not fit, by cp.async rows; no block-wide barrier in the loop.  Both
+// products are taken transposed, S^T = K Q^T and O^T += V^T P^T (m16n8k16), so that the 16-wide
+// side is full of keys or head elements and the 8-wide side holds the G rows: half the products and
+// registers of the other way round for G <= 8.  S^T turns into the second product's operand with
+// movmatrix.  The KS warps of a head join their (m, l, O) through shared memory when a request ends.
 constexpr int kDecodeWarps = 8;
 constexpr int kTile = 16;  // keys
 
 struct DecodeParams {
+  CUtensorMap kmap, vmap;
   AttentionParams a;
   Partials part;
   int n_ranges;        // equal runs of the page axis
   int hb_shift;        // log2 of the heads a CTA works on
   int units_per_page;  // 16-key units of a page
+  int box;             // keys of a TMA box
   long long slot0;     // first slot of the runs
   bool join_all;       // whole requests too go to a slot (behind the runs' own): a prefix follows
 };
 
-struct TileMeta {
-  int request;
-  int keys;   // keys of the tile that exist
-  int flags;  // 1: first tile of the request in this warp, 2: last
-  int slot;   // where the result goes: -1 = the output row (a slot is num_heads rows)
+struct __align__(16) TileMeta {
+  int request;  // -1: behind the last tile
+  int keys;     // keys of the tile that exist
+  int flags;    // 1: first tile of the request in this warp, 2: last
+  int slot;     // where the result goes: -1 = the output row (a slot is num_heads rows)
 };
 
 template <int D, int NST>
 struct DecodeSmem {
-  static constexpr int kRow = D * 2;
-  static constexpr int kStage = 2 * kTile * kRow;
+  static constexpr int kHalf = kTile * 128;             // 16 keys x 64 elements
+  static constexpr int kPlane = D / 64 * kHalf;
+  static constexpr int kStage = 2 * kPlane;
   static constexpr int kRing = kDecodeWarps * NST * kStage;
-  static constexpr int kMeta = kDecodeWarps * NST * (int)sizeof(TileMeta);
+  static constexpr int kMeta = kDecodeWarps * NST * (int)(sizeof(TileMeta) + sizeof(uint64_t));
   static int bytes(int G, int hb) {
     const int join = hb < kDecodeWarps ? kDecodeWarps * G * (D + 2) * 4 : 0;
-    return kRing + kMeta + join;
+    return 1024 + kRing + kMeta + join;
   }
 };
 
-template <bool BF16, int D, int NST>
-__global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(const DecodeParams p) {
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <bool BF16, int D, int NT, int NST, bool TMA>
+__global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(const __grid_constant__ DecodeParams p) {
   using S = DecodeSmem<D, NST>;
-  extern __shared__ __align__(128) char smem[];
-  constexpr int kSteps = D / 16, kChunks = D / 8;
+  extern __shared__ __align__(1024) char smem_raw[];
+  constexpr int kSteps = D / 16, kRowBytes = D * 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int HB = 1 << p.hb_shift, KS = kDecodeWarps >> p.hb_shift;
   const int hs = warp & (HB - 1), ks = warp >> p.hb_shift;
   const int kvh = blockIdx.y * HB + hs;
   const AttentionParams& a = p.a;
   const int G = a.num_heads / a.num_kv_heads;
-  const int UPP = p.units_per_page, BS = a.block_size;
+  const unsigned UPP = p.units_per_page, BS = a.block_size;
+  char* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t ring = smem_u32(smem) + warp * NST * S::kStage;
-  TileMeta* meta = reinterpret_cast<TileMeta*>(smem + S::kRing) + warp * NST;
-  float* joins = reinterpret_cast<float*>(smem + S::kRing + S::kMeta);
+  TileMeta* const meta = reinterpret_cast<TileMeta*>(smem + S::kRing) + warp * NST;
+  uint64_t* const full = reinterpret_cast<uint64_t*>(smem + S::kRing + kDecodeWarps * NST * sizeof(TileMeta)) + warp * NST;
+  float* const joins = reinterpret_cast<float*>(smem + S::kRing + S::kMeta);
 
+  if (TMA && lane < NST) mbar_init(&full[lane], 1);  // the warp's own
+  if (TMA) mbar_fence_init();
+  __syncwarp();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (kvh >= a.num_kv_heads) return;  // all KS warps of such a head slot leave together
 
-  // this CTA's run of units, [u_begin, u_end) of the page axis
-  const int* indptr = a.own.indptr;
+  // This CTA's run of units, [u_begin, u_end) of the page axis, and the request of its first unit:
+  // the last b with indptr[b] <= its page, 32 probes a round.
+  const int* const indptr = a.own.indptr;
   const int B = a.num_requests;
-  const long long axis0 = indptr[0];
-  const long long units = ((long long)indptr[B] - axis0) * UPP;
-  const long long chunk = (units + p.n_ranges - 1) / p.n_ranges;
-  const long long u_begin = chunk * blockIdx.x, u_end = min(u_begin + chunk, units);
-  if (u_begin >= u_end) return;
-
-  // the request of the first unit: the last b with indptr[b] <= its page, 32 probes a round
-  int b0 = 0;
+  unsigned u_begin, u_end;
+  int axis0, b0;
   {
-    const long long page = axis0 + u_begin / UPP;
-    int lo = 0, n = B;  // the answer is in [lo, lo + n)
+    int lo = 0, n = B, step = (n + 31) / 32;  // the answer is in [lo, lo + n)
+    int probe = lane * step < n ? indptr[lane * step] : 0;
+    axis0 = indptr[0];
+    const unsigned units = (unsigned)max(indptr[B] - axis0, 0) * UPP;
+    const unsigned chunk = (units + p.n_ranges - 1) / p.n_ranges;
+    u_begin = chunk * blockIdx.x;
+    u_end = min(u_begin + chunk, units);
+    if (u_begin >= u_end) return;
+    const int page = axis0 + (int)(u_begin / UPP);
     while (n > 1) {
-      const int step = (n + 31) / 32;
-      const int at = lo + lane * step;
-      const bool below = lane * step < n && indptr[at] <= page;
+      const bool below = lane * step < n && probe <= page;
       const int last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
       n = min(step, n - last * step);
       lo += last * step;
+      step = (n + 31) / 32;
+      probe = lane * step < n ? indptr[lo + lane * step] : 0;
     }
     b0 = lo;
   }
 
   // Producer: walks the requests of the run, 32 of them loaded at a time (one a lane).
-  int batch = b0, in_batch = -1;      // in_batch: index of the current request, -1 before the first
-  long long my_first = 0, my_end = 0; // lane's request: its pages on the axis
-  int my_last = 0;
+  int batch = b0, in_batch = -1;  // in_batch: index of the current request, -1 before the first
+  int my_first = 0, my_end = 0, my_last = 0;
   auto load_batch = [&]() {
     const int b = batch + lane;
-    my_first = my_end = 0;
-    my_last = 0;
+    my_first = my_end = my_last = 0;
     if (b < B) {
       my_first = indptr[b];
       my_end = indptr[b + 1];
-      my_last = min(max(a.own.last[b], 0), BS);
+      my_last = min(max(a.own.last[b], 0), (int)BS);
     }
   };
   load_batch();
@@ -306,270 +334,317 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
   int request = -1, slot = -1;
   bool fresh = false, done = false;          // fresh: no tile of the request issued yet
 
-  auto key_of = [&](long long unit) { return (long long)(unit / UPP) * BS + (unit % UPP) * kTile; };
+  auto key_of = [&](unsigned unit) { return (int)(unit / UPP * BS + unit % UPP * kTile); };
   auto next_request = [&]() {
     for (;;) {
       if (++in_batch == 32) {
         batch += 32;
         in_batch = 0;
-        if (batch >= B) { done = true; return; }
-        load_batch();
+        if (batch < B) load_batch();
       }
-      const long long first = __shfl_sync(0xffffffffu, my_first, in_batch);
-      const long long end = __shfl_sync(0xffffffffu, my_end, in_batch);
+      const int first = __shfl_sync(0xffffffffu, my_first, in_batch);
+      const int end = __shfl_sync(0xffffffffu, my_end, in_batch);
       const int last = __shfl_sync(0xffffffffu, my_last, in_batch);
       request = batch + in_batch;
-      if (request >= B) { done = true; return; }
-      const long long s0 = (first - axis0) * UPP, s1 = (end - axis0) * UPP;  // its units
-      if (s0 >= u_end) { done = true; return; }
+      const unsigned s0 = (unsigned)(first - axis0) * UPP, s1 = (unsigned)(end - axis0) * UPP;  // its units
+      if (request >= B || s0 >= u_end) { done = true; return; }
       if (end <= first || s1 <= u_begin) continue;
-      const long long len = (end - first - 1) * BS + last;
-      const long long k0 = s0 < u_begin ? key_of(u_begin - s0) : 0;
-      const long long k1 = s1 > u_end ? min(key_of(u_end - s0), len) : len;
-      key = (int)min(k0, len) + ks * kTile;
-      key_end = (int)k1;
-      first_page = (int)first;
-      const bool whole = s0 >= u_begin && s1 <= u_end;
-      slot = whole ? (p.join_all ? (int)p.slot0 + 2 * p.n_ranges + request : -1)
-                   : (int)p.slot0 + 2 * (int)blockIdx.x + (s0 < u_begin ? 0 : 1);
+      const int len = (end - first - 1) * (int)BS + last;
+      const int k0 = s0 < u_begin ? key_of(u_begin - s0) : 0;
+      key = min(k0, len) + ks * kTile;
+      key_end = s1 > u_end ? min(key_of(u_end - s0), len) : len;
+      first_page = first;
+      slot = s0 >= u_begin && s1 <= u_end ? (p.join_all ? (int)p.slot0 + 2 * p.n_ranges + request : -1)
+                                          : (int)p.slot0 + 2 * (int)blockIdx.x + (s0 < u_begin ? 0 : 1);
       fresh = true;
       return;
     }
   };
 
-  // Page numbers of the tile after the one being issued are fetched one tile ahead.
-  const long long head_off = (long long)kvh * S::kRow;
-  int row_page = 0;       // lane r < 16: page number of row r of the pending tile, -1 = none
-  int pend_key = 0, pend_flags = 0, pend_keys = 0, pend_request = 0, pend_slot = 0;
-  bool pending = false;
-  auto fetch = [&]() {  // describe the next tile and start loading its page numbers
-    pending = false;
+  // The next tile's description; its page numbers are on their way one tile before they are used.
+  int row_page = -1, row_entry = 0;  // lane r < 16: page and entry of row r, page -1 = none
+  TileMeta next = {-1, 0, 0, 0};
+  auto fetch = [&]() {
+    next.request = -1;
+    if (!done && (request < 0 || (!fresh && key >= key_end))) next_request();
     if (done) return;
-    if (request < 0 || (!fresh && key >= key_end)) next_request();
-    if (done) return;
-    pend_flags = fresh ? 1 : 0;
-    pend_request = request;
-    pend_slot = slot;
-    pend_key = key;
-    pend_keys = max(0, min(kTile, key_end - key));
-    key += KS * kTile;
-    if (key >= key_end) pend_flags |= 2;
+    next.request = request;
+    next.keys = max(0, min(kTile, key_end - key));
+    next.slot = slot;
+    next.flags = (fresh ? 1 : 0) | (key + KS * kTile >= key_end ? 2 : 0);
     fresh = false;
-    pending = true;
     row_page = -1;
-    if (lane < pend_keys) {
-      const long long at = (long long)first_page + (pend_key + lane) / BS;
+    if (lane < next.keys) {
+      const unsigned pg = (unsigned)(key + lane) / BS;
+      row_entry = key + lane - (int)(pg * BS);
+      const long long at = (long long)first_page + pg;
       if (at >= 0 && at < a.own.num_indices) {
         row_page = a.own.indices[at];
-        if (row_page < 0 || row_page >= a.num_blocks) {
+        if ((unsigned)row_page >= (unsigned)a.num_blocks) {
           if (a.checks) report(a.err, kErrBadPage, kWhereAttention, at, row_page);
-          row_page = -1;
+          row_page = -1;  // zeros
         }
       }
     }
+    key += KS * kTile;
   };
-  auto issue = [&](int stage) {  // start the pending tile's copies; always one commit
-    if (lane == 0) {
-      TileMeta m;
-      m.request = pending ? pend_request : -1;
-      m.keys = pend_keys;
-      m.flags = pend_flags;
-      m.slot = pend_slot;
-      meta[stage] = m;
-    }
-    if (pending) {
-      long long off = -1;
-      if (row_page >= 0)
-        off = (long long)row_page * a.block_stride + (long long)((pend_key + lane) % BS) * a.slot_stride + head_off;
-      const uint32_t base = ring + stage * S::kStage;
-      constexpr int kRowsAtOnce = 32 / kChunks;
-#pragma unroll
-      for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
-        const int row = i * kRowsAtOnce + lane / kChunks, c = lane % kChunks;
-        const long long o = __shfl_sync(0xffffffffu, off, row);
-        const uint32_t dst = base + row * S::kRow + ((c ^ (row & 7)) << 4);
-        const bool ok = o >= 0;
-        cp_async16(dst, ok ? a.kcache + o + c * 16 : a.kcache, ok);
-        cp_async16(dst + kTile * S::kRow, ok ? a.vcache + o + c * 16 : a.vcache, ok);
+  auto issue = [&](int stage) {  // starts the copies of the tile described by `next`
+    if (lane == 0) meta[stage] = next;
+    const uint32_t base = ring + stage * S::kStage;
+    if (TMA) {
+      if (next.request >= 0) {
+        const bool any = next.keys > 0;
+        if (lane == 0) {
+          if (any) mbar_expect_tx(&full[stage], S::kStage);
+          else mbar_arrive(&full[stage]);
+        }
+        __syncwarp();
+        constexpr int kBoxes = 2 * (D / 64);  // of one page: K and V, 64 elements each
+        const int piece = lane / kBoxes, plane = lane / (D / 64) & 1, half = lane % (D / 64);
+        const int src = piece * p.box;
+        const int page = __shfl_sync(0xffffffffu, row_page, src & 15);
+        const int entry = __shfl_sync(0xffffffffu, row_entry, src & 15);
+        if (any && src < kTile)
+          tma_load4(base + plane * S::kPlane + half * S::kHalf + src * 128, plane ? &p.vmap : &p.kmap, &full[stage],
+                    half * 64, page < 0 ? 0 : entry, kvh, page);
       }
+    } else {
+      if (next.request >= 0) {
+        long long off = -1;
+        if (row_page >= 0)
+          off = (long long)row_page * a.block_stride + (long long)row_entry * a.slot_stride + (long long)kvh * kRowBytes;
+        constexpr int kChunks = D / 8, kRowsAtOnce = 32 / kChunks;
+        const int c = lane % kChunks;
+#pragma unroll
+        for (int i = 0; i < kTile / kRowsAtOnce; ++i) {
+          const int row = i * kRowsAtOnce + lane / kChunks;
+          const long long o = __shfl_sync(0xffffffffu, off, row);
+          const uint32_t dst = base + (c >> 3) * S::kHalf + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+          const bool ok = o >= 0;
+          cp_async16(dst, ok ? a.kcache + o + c * 16 : a.kcache, ok);
+          cp_async16(dst + S::kPlane, ok ? a.vcache + o + c * 16 : a.vcache, ok);
+        }
+      }
+      cp_async_commit();
     }
-    cp_async_commit();
   };
 
   fetch();
 #pragma unroll
   for (int s = 0; s < NST - 1; ++s) {
     issue(s);
-    if (pending) fetch();
+    if (next.request >= 0) fetch();
   }
 
-  // Consumer
-  uint32_t q[kSteps][4];
-  float o[D / 8][4];
-  float m[2], l[2];
+  // Consumer.  A lane holds, of S^T, keys lane / 4 and lane / 4 + 8 of rows 2 (lane % 4) and the next;
+  // of O^T, elements 16 m + lane / 4 and + 8 of the same rows.
+  uint32_t q[kSteps][NT][2];
+  float o[kSteps][NT][4], m[NT][2], l[NT][2];
   const float scale2 = a.scale * kLog2e;
-  const int r0 = lane >> 2, c0 = (lane & 3) * 2;
-  for (int it = 0;; ++it) {
+  const int r0 = (lane & 3) * 2, e0 = lane >> 2;
+  // ldmatrix addresses inside a plane: row, then the lane's chunk of step 0; step k flips bits 5, 6
+  const uint32_t k_addr = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_addr = ((lane & 7) + ((lane >> 4) << 3)) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+  bool dead = false;
+  int it = 0;
+  for (;; ++it) {
     const int stage = it % NST;
-    cp_async_wait<NST - 2>();
+    if (!TMA) cp_async_wait<NST - 2>();
     __syncwarp();
     const TileMeta t = meta[stage];
     if (t.request < 0) break;
     issue((it + NST - 1) % NST);
-    if (pending) fetch();
+    if (next.request >= 0) fetch();
+    if (TMA && !dead && !mbar_wait_bounded(&full[stage], (it / NST) & 1)) {
+      report(a.err, kErrWaitTimeout, kWhereAttention, blockIdx.x, it);
+      dead = true;  // goes on without waiting: the head's other warps meet it at their barrier
+    }
 
     if (t.flags & 1) {
-      const char* rows = a.q + (long long)t.request * a.q_tok + (long long)kvh * G * S::kRow + c0 * 2;
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k)
+      for (int n = 0; n < NT; ++n) {
+        const bool row = n * 8 + e0 < G;
+        const char* src = a.q + (long long)t.request * a.q_tok + (long long)(kvh * G + n * 8 + e0) * kRowBytes + r0 * 2;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = r0 + (e & 1) * 8;
-          q[k][e] = r < G ? *reinterpret_cast<const uint32_t*>(rows + r * S::kRow + k * 32 + (e >> 1) * 16) : 0u;
+        for (int k = 0; k < kSteps; ++k) {
+          q[k][n][0] = row ? *reinterpret_cast<const uint32_t*>(src + k * 32) : 0u;
+          q[k][n][1] = row ? *reinterpret_cast<const uint32_t*>(src + k * 32 + 16) : 0u;
+          o[k][n][0] = o[k][n][1] = o[k][n][2] = o[k][n][3] = 0.f;
         }
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-      m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = 0.f;
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.f;
+      }
     }
 
     if (t.keys > 0) {
-      const uint32_t kbase = ring + stage * S::kStage, vbase = kbase + kTile * S::kRow;
-      float s[2][4] = {};
-      {
-        // matrices 0..3 of an ldmatrix: (keys 0-7, d lo) (keys 0-7, d hi) (keys 8-15, d lo) (keys 8-15, d hi)
-        const int row = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+      const uint32_t kbase = ring + stage * S::kStage, vbase = kbase + S::kPlane;
+      if (t.keys < kTile && TMA) {
+        // what lies behind the last key may be anything, and 0 * NaN is not 0
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          uint32_t b[4];
-          ldsm4(b, kbase + row * S::kRow + (((2 * k + half) ^ (row & 7)) << 4));
-          mma16816<BF16>(s[0], q[k], b[0], b[1]);
-          mma16816<BF16>(s[1], q[k], b[2], b[3]);
+        for (int c = lane; c < kTile * D / 8; c += 32) {
+          const int row = c / (D / 8), half = (c % (D / 8)) >> 3;
+          if (row >= t.keys)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vbase + half * S::kHalf + row * 128 + (c & 7) * 16), "r"(0) : "memory");
         }
+        fence_proxy_async();  // before the stage is filled again
+        __syncwarp();
       }
-      float top[2] = {m[0], m[1]};
+      float s[NT][4] = {};
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int k = 0; k < kSteps; ++k) {
+        uint32_t x[4];
+        ldsm4(x, kbase + (k >> 2) * S::kHalf + (k_addr ^ ((k & 3) << 5)));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool live = n * 8 + c0 + (e & 1) < t.keys;
-          s[n][e] = live ? s[n][e] * scale2 : -INFINITY;
-          top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+        for (int n = 0; n < NT; ++n) mma16816<BF16>(s[n], x, q[k][n][0], q[k][n][1]);
+      }
+      uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] *= scale2;
+        if (t.keys < kTile) {
+          if (e0 >= t.keys) s[n][0] = s[n][1] = -INFINITY;
+          if (e0 + 8 >= t.keys) s[n][2] = s[n][3] = -INFINITY;
         }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-      }
-      if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+        float keep[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float keep = m[i] == top[i] ? 1.f : exp2_fast(m[i] - top[i]);
-          m[i] = top[i];
-          l[i] *= keep;
-#pragma unroll
-          for (int n = 0; n < D / 8; ++n) {
-            o[n][2 * i] *= keep;
-            o[n][2 * i + 1] *= keep;
+          float top = fmaxf(s[n][i], s[n][2 + i]);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          keep[i] = 1.f;
+          if (top > m[n][i] + kLazy) {
+            keep[i] = exp2_fast(m[n][i] - top);
+            m[n][i] = top;
           }
         }
-      }
-      // The weights enter the second product in the element type, as a rounded part and the
-      // rounded rest: two products, error 2^-16 instead of 2^-8, on pipes that HBM leaves idle.
-      const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-      uint32_t hi[4], lo[4];
+        if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+          for (int k = 0; k < kSteps; ++k) {
+            o[k][n][0] *= keep[0];
+            o[k][n][1] *= keep[1];
+            o[k][n][2] *= keep[0];
+            o[k][n][3] *= keep[1];
+          }
+          l[n][0] *= keep[0];
+          l[n][1] *= keep[1];
+        }
+        // The weights enter the second product in the element type, as a rounded part and the
+        // rounded rest: two products, error 2^-16 instead of 2^-8, on pipes that HBM leaves idle.
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const float w0 = exp2_fast(s[n][2 * i] - base[i]), w1 = exp2_fast(s[n][2 * i + 1] - base[i]);
-          l[i] += w0 + w1;
-          hi[2 * n + i] = down2<BF16>(w0, w1);
-          const float2 h = up2<BF16>(hi[2 * n + i]);
-          lo[2 * n + i] = down2<BF16>(w0 - h.x, w1 - h.y);
+          const float w0 = exp2_fast(s[n][2 * i] - (m[n][0] == -INFINITY ? 0.f : m[n][0]));
+          const float w1 = exp2_fast(s[n][2 * i + 1] - (m[n][1] == -INFINITY ? 0.f : m[n][1]));
+          l[n][0] += w0;
+          l[n][1] += w1;
+          const uint32_t h = down2<BF16>(w0, w1);
+          const float2 f = up2<BF16>(h);
+          hi[n][i] = transpose8x8(h);
+          lo[n][i] = transpose8x8(down2<BF16>(w0 - f.x, w1 - f.y));
         }
-      {
-        // (keys 0-7, d n) (keys 8-15, d n) (keys 0-7, d n+1) (keys 8-15, d n+1), transposed
-        const int row = lane & 15, half = lane >> 4;
+      }
 #pragma unroll
-        for (int n = 0; n < D / 8; n += 2) {
-          uint32_t b[4];
-          ldsm4_t(b, vbase + row * S::kRow + (((n + half) ^ (row & 7)) << 4));
-          mma16816<BF16>(o[n], hi, b[0], b[1]);
-          mma16816<BF16>(o[n + 1], hi, b[2], b[3]);
-          mma16816<BF16>(o[n], lo, b[0], b[1]);
-          mma16816<BF16>(o[n + 1], lo, b[2], b[3]);
+      for (int k = 0; k < kSteps; ++k) {
+        uint32_t x[4];
+        ldsm4_t(x, vbase + (k >> 2) * S::kHalf + (v_addr ^ ((k & 3) << 5)));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma16816<BF16>(o[k][n], x, hi[n][0], hi[n][1]);
+          mma16816<BF16>(o[k][n], x, lo[n][0], lo[n][1]);
         }
       }
     }
 
     if (t.flags & 2) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-      }
       const int head0 = kvh * G;
-      char* out = a.out + (long long)t.request * a.o_tok + (long long)head0 * S::kRow;
-      float* lse = t.slot >= 0 ? p.part.lse + (long long)t.slot * a.num_heads + head0
-                   : a.lse != nullptr ? a.lse + (long long)t.request * a.num_heads + head0 : nullptr;
-      float* po = p.part.out + ((long long)max(t.slot, 0) * a.num_heads + head0) * D;
+      char* const out = a.out + (long long)t.request * a.o_tok + (long long)head0 * kRowBytes;
+      float* const lse = t.slot >= 0 ? p.part.lse + (long long)t.slot * a.num_heads + head0
+                         : a.lse != nullptr ? a.lse + (long long)t.request * a.num_heads + head0 : nullptr;
+      float* const po = p.part.out + ((long long)max(t.slot, 0) * a.num_heads + head0) * D;
       const float unit = t.slot >= 0 ? 1.f : kLn2;  // partials keep base 2
-      if (KS == 1) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int r = r0 + 8 * i;
-          if (r >= G) continue;
-          const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
-          if (lse != nullptr && c0 == 0) lse[r] = l[i] > 0.f ? (m[i] + log2f(l[i])) * unit : -INFINITY;
+          l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], 4);
+          l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], 8);
+          l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], 16);
+        }
+      if (KS == 1) {
 #pragma unroll
-          for (int n = 0; n < D / 8; ++n) {
-            const float x = o[n][2 * i] * inv, y = o[n][2 * i + 1] * inv;
-            if (t.slot >= 0) *reinterpret_cast<float2*>(po + r * D + n * 8 + c0) = make_float2(x, y);
-            else *reinterpret_cast<uint32_t*>(out + r * S::kRow + (n * 8 + c0) * 2) = down2<BF16>(x, y);
+        for (int n = 0; n < NT; ++n) {
+          float inv[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = n * 8 + r0 + i;
+            inv[i] = l[n][i] > 0.f ? 1.f / l[n][i] : (l[n][i] == 0.f ? 0.f : l[n][i]);
+            if (lse != nullptr && e0 == 0 && r < G) lse[r] = l[n][i] == 0.f ? -INFINITY : (m[n][i] + log2f(l[n][i])) * unit;
           }
+#pragma unroll
+          for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float x = o[k][n][2 * h] * inv[0], y = o[k][n][2 * h + 1] * inv[1];
+              const int d = 16 * k + 8 * h;
+              if (t.slot >= 0) {
+                const int r = n * 8 + r0;
+                if (r < G) po[r * D + d + e0] = x;
+                if (r + 1 < G) po[(r + 1) * D + d + e0] = y;
+              } else {
+                const uint32_t v = transpose8x8(down2<BF16>(x, y));  // row lane / 4, two elements
+                if (n * 8 + e0 < G) *reinterpret_cast<uint32_t*>(out + (n * 8 + e0) * kRowBytes + (d + r0) * 2) = v;
+              }
+            }
         }
       } else {
         // [warp][G][D] accumulators, then [warp][G] maxima and sums
-        float* jm = joins + kDecodeWarps * G * D;
-        float* jl = jm + kDecodeWarps * G;
+        float* const jm = joins + kDecodeWarps * G * D;
+        float* const jl = jm + kDecodeWarps * G;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = r0 + 8 * i;
-          if (r >= G) continue;
-          if (c0 == 0) {
-            jm[warp * G + r] = m[i];
-            jl[warp * G + r] = l[i];
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = n * 8 + r0 + i;
+            if (r >= G) continue;
+            if (e0 == 0) {
+              jm[warp * G + r] = m[n][i];
+              jl[warp * G + r] = l[n][i];
+            }
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+              joins[(warp * G + r) * D + 16 * k + e0] = o[k][n][i];
+              joins[(warp * G + r) * D + 16 * k + 8 + e0] = o[k][n][2 + i];
+            }
           }
-#pragma unroll
-          for (int n = 0; n < D / 8; ++n)
-            *reinterpret_cast<float2*>(joins + (warp * G + r) * D + n * 8 + c0) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
-        }
         asm volatile("bar.sync %0, %1;" ::"r"(1 + hs), "r"(KS * 32) : "memory");
         for (int e = ks * 32 + lane; e < G * (D / 2); e += KS * 32) {
           const int r = e / (D / 2), d = (e - r * (D / 2)) * 2;
           float mm = -INFINITY;
           for (int k = 0; k < KS; ++k) mm = fmaxf(mm, jm[(hs + k * HB) * G + r]);
           float ll = 0.f, x = 0.f, y = 0.f;
-          if (mm != -INFINITY)
-            for (int k = 0; k < KS; ++k) {
-              const int w = (hs + k * HB) * G + r;
-              const float f = exp2_fast(jm[w] - mm);
-              const float2 v = *reinterpret_cast<const float2*>(joins + w * D + d);
-              ll = fmaf(f, jl[w], ll);
-              x = fmaf(f, v.x, x);
-              y = fmaf(f, v.y, y);
-            }
-          const float inv = ll > 0.f ? 1.f / ll : 0.f;
+          for (int k = 0; k < KS; ++k) {
+            const int w = (hs + k * HB) * G + r;
+            const float f = jm[w] == -INFINITY ? 0.f : exp2_fast(jm[w] - mm);
+            const float2 v = *reinterpret_cast<const float2*>(joins + w * D + d);
+            ll = fmaf(f, jl[w], ll);
+            x = fmaf(f, v.x, x);
+            y = fmaf(f, v.y, y);
+          }
+          const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
           if (t.slot >= 0) *reinterpret_cast<float2*>(po + r * D + d) = make_float2(x * inv, y * inv);
-          else *reinterpret_cast<uint32_t*>(out + r * S::kRow + d * 2) = down2<BF16>(x * inv, y * inv);
-          if (d == 0 && lse != nullptr) lse[r] = ll > 0.f ? (mm + log2f(ll)) * unit : -INFINITY;
+          else *reinterpret_cast<uint32_t*>(out + r * kRowBytes + d * 2) = down2<BF16>(x * inv, y * inv);
+          if (d == 0 && lse != nullptr) lse[r] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * unit;
         }
         asm volatile("bar.sync %0, %1;" ::"r"(1 + hs), "r"(KS * 32) : "memory");
       }
     }
   }
-  cp_async_wait<0>();
+  if (!TMA) cp_async_wait<0>();
+  // Every tile issued was also waited for, unless a wait ran out: then once more, so that no copy
+  // is in flight when the CTA leaves.
+  if (TMA && dead)
+    for (int i = max(0, it - NST); i < it; ++i) mbar_wait_bounded(&full[i % NST], (i / NST) & 1);
 }
 
 // ---------------------------------------------------------------- tiles of rows
@@ -585,7 +660,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
 //                    one row tile's softmax runs beside the other's products
 //
 // The maximum is only moved (and O rescaled in tensor memory, by the softmax threads) when it
-// grows by more than 2^8: P and l may exceed 1 by that factor, which fp32 sums and 16-bit P hold.
+// grows by more than 8 in base 2: P and l may exceed 1 by that factor, which fp32 sums and 16-bit P hold.
 // S of the next tile overwrites P: it is issued behind the PV that reads it, and the commit behind
 // it tells the softmax warps that this PV, too, is complete.  P is rounded to the element type
 // (half a step, 2^-8 in bf16): the tensor cores take no wider second operand.
@@ -597,7 +672,6 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
 constexpr int kRows = 128;       // rows of a tile
 constexpr int kKeys = 128;       // keys of a tile
 constexpr int kTileThreads = 384;
-constexpr float kLazy = 8.f;     // log2 of the factor the maximum may lag behind
 
 struct TileParams {
   CUtensorMap kmap, vmap;
@@ -626,10 +700,6 @@ struct TileBars {
   int dead;
 };
 
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
@@ -685,12 +755,6 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint
       "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
       "r"(add ? 1u : 0u)
-      : "memory");
-}
-__device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
 }
 
@@ -845,7 +909,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   const uint32_t tmem = bars.tmem;
   const uint32_t sm_q = smem + S::kQ, sm_k = smem + S::kK, sm_v = smem + S::kV;
   const int first_page = p.list.indptr[seq];
-  const float scale2 = fabsf(a.scale) * kLog2e;
+  // The sign of the scale goes into Q; a scale of 0 must still leave masked scores at -infinity.
+  const float scale2 = fmaxf(fabsf(a.scale) * kLog2e, 1.1754944e-38f);
 
   // A wait that runs out ends the role; the others run out in turn, and the CTA leaves in order.
   auto wait = [&](uint64_t* bar, unsigned parity) -> bool {
@@ -1062,7 +1127,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
 // ---------------------------------------------------------------- join
 // One warp a row: the row's partials, weighted by 2^(lse - max lse).  Sets [0, n_shared) come from
 // the prefix, [n_shared, n_sets) from the own keys, one slot a token each; behind them the slots of
-// the decode kernel's runs.
+// the decode kernel's runs.  A lane looks up the lse of one part, so the parts' weights are known
+// before the first of them is read and their loads do not wait for one another.
 struct JoinParams {
   AttentionParams a;
   Partials part;
@@ -1071,30 +1137,17 @@ struct JoinParams {
   bool all;         // its whole requests, too, lie in slots
   int n_ranges, units_per_page;
 };
+constexpr int kJoinWarps = 8;
 
 template <bool BF16, int D>
-__global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const JoinParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const AttentionParams& a = p.a;
   const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int t = (int)(row / a.num_heads), h = (int)(row - (long long)t * a.num_heads);
-  if (t >= a.num_tokens) return;
-  constexpr int E = D / 32;
-  float acc[E] = {}, m = -INFINITY, l = 0.f;
-  auto add = [&](long long slot) {
-    const long long at = slot * a.num_heads + h;
-    const float s = p.part.lse[at];
-    if (s == -INFINITY) return;
-    const float top = fmaxf(m, s), keep = exp2_fast(m - top), w = exp2_fast(s - top);
-    m = top;
-    l = l * keep + w;
-    const float* v = p.part.out + at * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(w, v[e], acc[e] * keep);
-  };
-  int first = 0;
+  const int t = blockIdx.x, h = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
+  if (h >= a.num_heads) return;
+  int first = 0;  // parts of the row: sets [first, n_sets), then n_runs slots of the runs
   if (a.qo_indptr != nullptr && (t < a.qo_indptr[0] || t >= a.qo_indptr[a.num_requests])) return;  // left as it is
   if (p.n_shared > 0 && a.group_indptr != nullptr) {
     // a request outside every group has no set from the prefix
@@ -1103,30 +1156,72 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const JoinParams p)
     const int t0 = a.qo_indptr != nullptr ? a.qo_indptr[b0] : b0, t1 = a.qo_indptr != nullptr ? a.qo_indptr[b1] : b1;
     if (t < t0 || t >= t1) first = p.n_shared;
   }
+  const long long slot0 = (long long)p.n_sets * a.num_tokens;
+  int n_runs = 0, x0 = 0;
   if (p.runs) {
     const int* indptr = a.own.indptr;
-    const long long axis0 = indptr[0];
-    const long long units = ((long long)indptr[a.num_requests] - axis0) * p.units_per_page;
-    const long long chunk = (units + p.n_ranges - 1) / p.n_ranges;
-    const long long s0 = (indptr[t] - axis0) * p.units_per_page, s1 = (indptr[t + 1] - axis0) * p.units_per_page;
-    const long long slot0 = (long long)p.n_sets * a.num_tokens;
-    if (s1 > s0 && chunk > 0) {  // the runs that hold a part of the request
-      const int x0 = (int)min(max(s0 / chunk, 0ll), p.n_ranges - 1ll);
-      const int x1 = (int)min(max((s1 - 1) / chunk, 0ll), p.n_ranges - 1ll);
-      if (x0 == x1) {
-        if (!p.all) return;  // finished by its run
-        add(slot0 + 2 * p.n_ranges + t);
-      } else {
-        for (int x = x0; x <= x1; ++x) add(slot0 + 2 * x + (x == x0 ? 1 : 0));
-      }
+    const int axis0 = indptr[0], begin = indptr[t], end = indptr[t + 1];
+    const unsigned units = (unsigned)max(indptr[a.num_requests] - axis0, 0) * p.units_per_page;
+    const unsigned chunk = (units + p.n_ranges - 1) / p.n_ranges;
+    if (end > begin && chunk > 0) {  // the runs that hold a part of the request
+      x0 = (int)min((unsigned)(begin - axis0) * p.units_per_page / chunk, p.n_ranges - 1u);
+      n_runs = (int)min(((unsigned)(end - axis0) * p.units_per_page - 1) / chunk, p.n_ranges - 1u) - x0 + 1;
+      if (n_runs == 1 && !p.all) return;  // finished by its run
     }
   }
-  for (int x = first; x < p.n_sets; ++x) add((long long)x * a.num_tokens + t);
+  const int n_set = p.n_sets - first, n = n_set + max(n_runs, 0);
+  auto slot_of = [&](int i) -> long long {
+    if (i < n_set) return (long long)(first + i) * a.num_tokens + t;
+    if (n_runs == 1) return slot0 + 2 * p.n_ranges + t;  // whole
+    const int x = i - n_set;
+    return slot0 + 2 * (x0 + x) + (x == 0 ? 1 : 0);
+  };
+  constexpr int E = D / 32;
+  float acc[E] = {}, m = -INFINITY, l = 0.f;
+  for (int base = 0; base < n; base += 32) {
+    long long at = 0;
+    float s = -INFINITY;
+    if (base + lane < n) {
+      at = slot_of(base + lane) * a.num_heads + h;
+      s = p.part.lse[at];
+    }
+    float top = fmaxf(s, m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float w = s == -INFINITY ? 0.f : exp2_fast(s - top);  // a part without a key was not written
+    if (m != -INFINITY) {
+      const float keep = exp2_fast(m - top);
+      l *= keep;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= keep;
+    }
+    m = top;
+    const unsigned live = __ballot_sync(0xffffffffu, w != 0.f);
+#pragma unroll 4
+    for (int i = 0; i < min(32, n - base); ++i) {
+      const float wi = __shfl_sync(0xffffffffu, w, i);
+      const long long ai = __shfl_sync(0xffffffffu, at, i);
+      l += wi;
+      float v[E] = {};
+      if (live >> i & 1) {
+        if constexpr (E == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(p.part.out + ai * D + lane * E);
+          v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        } else {
+          const float2 x = *reinterpret_cast<const float2*>(p.part.out + ai * D + lane * E);
+          v[0] = x.x; v[1] = x.y;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(wi, v[e], acc[e]);
+    }
+  }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   uint32_t* out = reinterpret_cast<uint32_t*>(a.out + (long long)t * a.o_tok + ((long long)h * D + lane * E) * 2);
 #pragma unroll
   for (int e = 0; e < E; e += 2) out[e / 2] = down2<BF16>(acc[e] * inv, acc[e + 1] * inv);
-  if (a.lse != nullptr && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (a.lse != nullptr && lane == 0)
+    a.lse[(long long)t * a.num_heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // ---------------------------------------------------------------- launch rules
@@ -1205,25 +1300,6 @@ struct Launch {
   }
 };
 
-template <bool BF16, int D, int NST>
-cudaError_t launch_decode(const AttentionParams& p, const Plan& plan, bool pdl, cudaStream_t stream) {
-  DecodeParams d{};
-  d.a = p;
-  d.part = partials_at(p, plan);
-  d.n_ranges = plan.n_ranges;
-  d.hb_shift = plan.hb_shift;
-  d.units_per_page = plan.units_per_page;
-  d.slot0 = (long long)(plan.shared_splits + plan.own_splits) * p.num_tokens;
-  d.join_all = plan.shared_splits > 0;
-  const int G = p.num_heads / p.num_kv_heads, HB = 1 << plan.hb_shift;
-  auto kernel = attention_decode_kernel<BF16, D, NST>;
-  const int smem = DecodeSmem<D, NST>::bytes(G, HB);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  Launch go(dim3(plan.n_ranges, (p.num_kv_heads + HB - 1) / HB), kDecodeWarps * 32, smem, pdl, stream);
-  return cudaLaunchKernelEx(&go.cfg, kernel, d);
-}
-
 // The driver's encoder, through the runtime (the library links no libcuda).
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -1251,6 +1327,27 @@ bool encode_plane(const AttentionParams& p, const char* base, int box, CUtensorM
   return fn(map, p.is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<char*>(base),
             dims, strides, box_dims, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool BF16, int D, int NT, int NST>
+cudaError_t launch_decode(const AttentionParams& p, const Plan& plan, bool pdl, cudaStream_t stream) {
+  DecodeParams d{};
+  d.a = p;
+  d.part = partials_at(p, plan);
+  d.n_ranges = plan.n_ranges;
+  d.hb_shift = plan.hb_shift;
+  d.units_per_page = plan.units_per_page;
+  d.slot0 = (long long)(plan.shared_splits + plan.own_splits) * p.num_tokens;
+  d.join_all = plan.shared_splits > 0;
+  const int G = p.num_heads / p.num_kv_heads, HB = 1 << plan.hb_shift;
+  d.box = p.block_size % kTile == 0 ? kTile : p.block_size == 8 ? 8 : 0;
+  const bool tma = d.box > 0 && encode_plane(p, p.kcache, d.box, &d.kmap) && encode_plane(p, p.vcache, d.box, &d.vmap);
+  auto kernel = tma ? attention_decode_kernel<BF16, D, NT, NST, true> : attention_decode_kernel<BF16, D, NT, NST, false>;
+  const int smem = DecodeSmem<D, NST>::bytes(G, HB);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  Launch go(dim3(plan.n_ranges, (p.num_kv_heads + HB - 1) / HB), kDecodeWarps * 32, smem, pdl, stream);
+  return cudaLaunchKernelEx(&go.cfg, kernel, d);
 }
 
 template <bool BF16, int D>
@@ -1291,9 +1388,7 @@ cudaError_t launch_join(const AttentionParams& p, const Plan& plan, bool pdl, cu
   j.all = plan.shared_splits > 0;
   j.n_ranges = plan.n_ranges;
   j.units_per_page = plan.units_per_page;
-  const long long ctas = ((long long)p.num_tokens * p.num_heads + 3) / 4;
-  if (ctas > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  Launch go(dim3((unsigned)ctas), 128, 0, pdl, stream);
+  Launch go(dim3(p.num_tokens, (p.num_heads + kJoinWarps - 1) / kJoinWarps), kJoinWarps * 32, 0, pdl, stream);
   return cudaLaunchKernelEx(&go.cfg, attention_join_kernel<BF16, D>, j);
 }
 
@@ -1314,9 +1409,8 @@ cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, bool pdl, 
   }
   if (e == cudaSuccess && plan.runs) {
     const bool few = p.num_heads / p.num_kv_heads <= 8;
-    e = D == 64 ? launch_decode<BF16, 64, 5>(p, plan, pdl, stream)
-        : few   ? launch_decode<BF16, 128, 3>(p, plan, pdl, stream)
-                : launch_decode<BF16, 128, 2>(p, plan, pdl, stream);
+    constexpr int kDeep = D == 64 ? 6 : 3;
+    e = few ? launch_decode<BF16, D, 1, kDeep>(p, plan, pdl, stream) : launch_decode<BF16, D, 2, D == 64 ? 5 : 2>(p, plan, pdl, stream);
     *launches += e == cudaSuccess;
   } else if (e == cudaSuccess) {
     e = launch_tile<BF16, D>(p, plan, false, pdl, stream);

@@ -175,6 +175,13 @@ def test_flat_and_peaked_scores(spread):
 
 
 @gpu
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-4])
+@pytest.mark.parametrize("new", [None, [3, 60, 1]])
+def test_scales_of_any_sign(scale, new):
+    check(case([100, 60, 3], new, prefix=[50]), scale=scale)
+
+
+@gpu
 def test_rising_scores_move_the_running_maximum():
     # every key scores higher than the ones before it, across all tile borders
     c = case([600, 400], [70, 1], HQ=2, H=1, D=64, dtype=HF)
