@@ -293,26 +293,36 @@ int lms_rope_and_cache(const void* query, const void* key, const void* value,
  * and K before they rotate it.  For every head x of Q and K, with w = query_weight / key_weight
  * ([head_dim], shared by the heads):
  *   n = x * w / sqrt(mean(x^2) + eps),   then the two lines of lms_rope_and_cache on n,
- * evaluated in fp32 and rounded once.  Arguments, layouts and the slot < 0 padding rule are those
- * of lms_rope_and_cache, with two differences: max_position and (with a cache) num_slots are
+ * evaluated in fp32 and rounded once.  The fields, layouts and the slot < 0 padding rule are those
+ * of the arguments of lms_rope_and_cache, with two differences: max_position and (with a cache) num_slots are
  * required and always enforced - a token whose position is outside the table gets no rotated Q
  * and no K, one whose slot is outside the cache no cache row; the debug checks report it - and
  * head_dim is a multiple of 16 up to 512.  (The reference has no such model; the call takes the
  * place of rotary_pos_emb at runtime/worker/llm_worker/models/llama.py:156-167.)
  */
-int lms_qk_norm_rope_and_cache(const void* query, const void* key, const void* value,
-                               int64_t query_token_stride, int64_t key_token_stride,
-                               int64_t value_token_stride, const void* query_weight,
-                               const void* key_weight, double eps, const void* positions,
-                               int32_t positions_are_int64, const void* cos_sin_cache,
-                               int64_t cos_sin_row_stride, void* q_out,
-                               int64_t q_out_token_stride, void* k_out,
-                               int64_t k_out_token_stride, void* key_cache,
-                               void* value_cache, int64_t block_stride, int64_t slot_stride,
-                               const int64_t* slot_mapping, int64_t num_tokens,
-                               int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                               int32_t dtype, int32_t block_size, int64_t num_slots,
-                               int64_t max_position, void* stream);
+typedef struct lms_qk_norm_args {
+  const void* query;
+  const void* key;
+  const void* value;
+  int64_t query_token_stride, key_token_stride, value_token_stride;
+  const void* query_weight;
+  const void* key_weight;
+  double eps;
+  const void* positions;
+  int64_t positions_are_int64;
+  const void* cos_sin_cache;
+  int64_t cos_sin_row_stride;
+  void* q_out;
+  int64_t q_out_token_stride;
+  void* k_out;
+  int64_t k_out_token_stride;
+  void* key_cache;
+  void* value_cache;
+  int64_t block_stride, slot_stride;
+  const int64_t* slot_mapping;
+  int64_t num_tokens, num_heads, num_kv_heads, head_dim, dtype, block_size, num_slots, max_position;
+} lms_qk_norm_args;
+int lms_qk_norm_rope_and_cache(const lms_qk_norm_args* args, void* stream);
 
 /*
  * Attention of a batch over its pages of one layer's cache - the call of

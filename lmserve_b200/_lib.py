@@ -6,7 +6,7 @@ symbol the header declares, importing this module's ``lib()`` raises.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_double, c_int, c_int32, c_int64, c_void_p, POINTER
+from ctypes import c_char_p, c_int, c_int32, c_int64, c_void_p, POINTER
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "liblmserve_kv.so"
@@ -82,11 +82,7 @@ SIGNATURES = {
         c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,
         c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int64,
         c_void_p]),
-    "lms_qk_norm_rope_and_cache": (c_int, [
-        c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_double,
-        c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
-        c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32,
-        c_int64, c_int64, c_void_p]),
+    "lms_qk_norm_rope_and_cache": (c_int, [c_void_p, c_void_p]),
     "lms_attention_workspace_bytes": (c_int64, [c_void_p]),
     "lms_paged_attention": (c_int, [c_void_p, c_void_p]),
     "lms_build_step_indices": (c_int, [

@@ -745,74 +745,63 @@ int lms_rope_and_cache(const void* query, const void* key, const void* value,
   return LMS_OK;
 }
 
-int lms_qk_norm_rope_and_cache(const void* query, const void* key, const void* value,
-                               int64_t query_token_stride, int64_t key_token_stride,
-                               int64_t value_token_stride, const void* query_weight,
-                               const void* key_weight, double eps, const void* positions,
-                               int32_t positions_are_int64, const void* cos_sin_cache,
-                               int64_t cos_sin_row_stride, void* q_out,
-                               int64_t q_out_token_stride, void* k_out,
-                               int64_t k_out_token_stride, void* key_cache,
-                               void* value_cache, int64_t block_stride, int64_t slot_stride,
-                               const int64_t* slot_mapping, int64_t num_tokens,
-                               int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                               int32_t dtype, int32_t block_size, int64_t num_slots,
-                               int64_t max_position, void* stream) {
-  if (num_tokens < 0 || num_tokens > 0x7fffffffll || num_heads <= 0 || num_kv_heads <= 0 ||
-      num_heads > (1 << 20) || num_kv_heads > (1 << 20) || head_dim <= 0 || num_slots < 0 ||
-      max_position < 0 || (dtype != 0 && dtype != 1) || !(eps >= 0.0) || eps > 1e30)
+int lms_qk_norm_rope_and_cache(const lms_qk_norm_args* a, void* stream) {
+  if (!a) return LMS_ERR_NULL;
+  if (a->num_tokens < 0 || a->num_tokens > 0x7fffffffll || a->num_heads <= 0 || a->num_kv_heads <= 0 ||
+      a->num_heads > (1 << 20) || a->num_kv_heads > (1 << 20) || a->head_dim <= 0 || a->num_slots < 0 ||
+      a->max_position < 0 || (a->dtype != 0 && a->dtype != 1) || !(a->eps >= 0.0) || a->eps > 1e30)
     return LMS_ERR_RANGE;
-  if (head_dim % 16 != 0 || head_dim > 512) return LMS_ERR_UNSUPPORTED;
-  if (num_tokens == 0) return LMS_OK;
-  const bool cached = key_cache != nullptr || value_cache != nullptr;
-  if (!query || !key || !query_weight || !key_weight || !positions || !cos_sin_cache || !q_out)
+  if (a->head_dim % 16 != 0 || a->head_dim > 512) return LMS_ERR_UNSUPPORTED;
+  if (a->num_tokens == 0) return LMS_OK;
+  const bool cached = a->key_cache != nullptr || a->value_cache != nullptr;
+  if (!a->query || !a->key || !a->query_weight || !a->key_weight || !a->positions || !a->cos_sin_cache ||
+      !a->q_out)
     return LMS_ERR_NULL;
-  if (cached && (!key_cache || !value_cache || !value || !slot_mapping)) return LMS_ERR_NULL;
-  if (cached && block_size <= 0) return LMS_ERR_RANGE;
-  if (!ptr16(query) || !ptr16(key) || !ptr16(query_weight) || !ptr16(key_weight) ||
-      !ptr16(cos_sin_cache) || !ptr16(q_out) || !ptr16(k_out) || !mult16(query_token_stride) ||
-      !mult16(key_token_stride) || !mult16(cos_sin_row_stride) || !mult16(q_out_token_stride) ||
-      !mult16(k_out_token_stride) ||
-      ((uintptr_t)positions & (positions_are_int64 ? 7u : 3u)) != 0)
+  if (cached && (!a->key_cache || !a->value_cache || !a->value || !a->slot_mapping)) return LMS_ERR_NULL;
+  if (cached && (a->block_size <= 0 || a->block_size > 0x7fffffffll)) return LMS_ERR_RANGE;
+  if (!ptr16(a->query) || !ptr16(a->key) || !ptr16(a->query_weight) || !ptr16(a->key_weight) ||
+      !ptr16(a->cos_sin_cache) || !ptr16(a->q_out) || !ptr16(a->k_out) || !mult16(a->query_token_stride) ||
+      !mult16(a->key_token_stride) || !mult16(a->cos_sin_row_stride) || !mult16(a->q_out_token_stride) ||
+      !mult16(a->k_out_token_stride) || ((uintptr_t)a->positions & (a->positions_are_int64 ? 7u : 3u)) != 0)
     return LMS_ERR_ALIGN;
-  if (cached && (!ptr16(value) || !ptr16(key_cache) || !ptr16(value_cache) ||
-                 !mult16(value_token_stride) || !mult16(block_stride) ||
-                 !mult16(slot_stride) || ((uintptr_t)slot_mapping & 7u) != 0))
+  if (cached && (!ptr16(a->value) || !ptr16(a->key_cache) || !ptr16(a->value_cache) ||
+                 !mult16(a->value_token_stride) || !mult16(a->block_stride) || !mult16(a->slot_stride) ||
+                 ((uintptr_t)a->slot_mapping & 7u) != 0))
     return LMS_ERR_ALIGN;
 
   DeviceState* ds = nullptr;
   if (int rc = device_state(&ds)) return rc;
   QkNormRopeParams p{};
-  p.q = (const char*)query;
-  p.k = (const char*)key;
-  p.v = (const char*)value;
-  p.q_tok = query_token_stride;
-  p.k_tok = key_token_stride;
-  p.v_tok = value_token_stride;
-  p.q_weight = (const char*)query_weight;
-  p.k_weight = (const char*)key_weight;
-  p.eps = (float)eps;
-  p.positions = positions;
-  p.pos64 = positions_are_int64 ? 1 : 0;
-  p.cos_sin = (const char*)cos_sin_cache;
-  p.cs_row = cos_sin_row_stride;
-  p.q_out = (char*)q_out;
-  p.qo_tok = q_out_token_stride;
-  p.k_out = (char*)k_out;
-  p.ko_tok = k_out_token_stride;
-  p.kcache = cached ? (char*)key_cache : nullptr;
-  p.vcache = cached ? (char*)value_cache : nullptr;
-  p.block_stride = block_stride;
-  p.slot_stride = slot_stride;
-  p.slots = (const long long*)slot_mapping;
-  p.num_slots = num_slots;
-  p.max_pos = max_position;
-  p.num_tokens = (int)num_tokens;
-  p.num_heads = num_heads;
-  p.num_kv_heads = num_kv_heads;
-  p.head_dim = head_dim;
-  p.block_size = cached ? block_size : 1;
-  p.is_bf16 = dtype;
+  p.q = (const char*)a->query;
+  p.k = (const char*)a->key;
+  p.v = (const char*)a->value;
+  p.q_tok = a->query_token_stride;
+  p.k_tok = a->key_token_stride;
+  p.v_tok = a->value_token_stride;
+  p.q_weight = (const char*)a->query_weight;
+  p.k_weight = (const char*)a->key_weight;
+  p.eps = (float)a->eps;
+  p.positions = a->positions;
+  p.pos64 = a->positions_are_int64 ? 1 : 0;
+  p.cos_sin = (const char*)a->cos_sin_cache;
+  p.cs_row = a->cos_sin_row_stride;
+  p.q_out = (char*)a->q_out;
+  p.qo_tok = a->q_out_token_stride;
+  p.k_out = (char*)a->k_out;
+  p.ko_tok = a->k_out_token_stride;
+  p.kcache = cached ? (char*)a->key_cache : nullptr;
+  p.vcache = cached ? (char*)a->value_cache : nullptr;
+  p.block_stride = a->block_stride;
+  p.slot_stride = a->slot_stride;
+  p.slots = (const long long*)a->slot_mapping;
+  p.num_slots = a->num_slots;
+  p.max_pos = a->max_position;
+  p.num_tokens = (int)a->num_tokens;
+  p.num_heads = (int)a->num_heads;
+  p.num_kv_heads = (int)a->num_kv_heads;
+  p.head_dim = (int)a->head_dim;
+  p.block_size = cached ? (int)a->block_size : 1;
+  p.is_bf16 = (int)a->dtype;
   p.err = ds->err.load(std::memory_order_relaxed);
   p.checks = g_checks.load(std::memory_order_relaxed);
   LMS_CUDA(launch_qk_norm_rope(p, ds->sms, tuned(LMS_TUNE_WRITE_PDL, 1) == 1, (cudaStream_t)stream));

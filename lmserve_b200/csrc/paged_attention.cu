@@ -11,6 +11,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "kernels.cuh"
 
 namespace lms {
@@ -1329,6 +1331,19 @@ bool encode_plane(const AttentionParams& p, const char* base, int box, CUtensorM
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Shared memory beyond the default has to be asked for, once per kernel and device.
+template <class K>
+cudaError_t allow_smem(K kernel, int most, std::atomic<unsigned long long>* asked) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (asked->load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess) asked->fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
 template <bool BF16, int D, int NT, int NST>
 cudaError_t launch_decode(const AttentionParams& p, const Plan& plan, bool pdl, cudaStream_t stream) {
   DecodeParams d{};
@@ -1344,7 +1359,8 @@ cudaError_t launch_decode(const AttentionParams& p, const Plan& plan, bool pdl, 
   const bool tma = d.box > 0 && encode_plane(p, p.kcache, d.box, &d.kmap) && encode_plane(p, p.vcache, d.box, &d.vmap);
   auto kernel = tma ? attention_decode_kernel<BF16, D, NT, NST, true> : attention_decode_kernel<BF16, D, NT, NST, false>;
   const int smem = DecodeSmem<D, NST>::bytes(G, HB);
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<unsigned long long> asked[2];
+  cudaError_t e = allow_smem(kernel, DecodeSmem<D, NST>::bytes(8 * NT, 1), &asked[tma]);
   if (e != cudaSuccess) return e;
   Launch go(dim3(plan.n_ranges, (p.num_kv_heads + HB - 1) / HB), kDecodeWarps * 32, smem, pdl, stream);
   return cudaLaunchKernelEx(&go.cfg, kernel, d);
@@ -1371,7 +1387,8 @@ cudaError_t launch_tile(const AttentionParams& p, const Plan& plan, bool shared,
   if (t.box > 0 && !(encode_plane(p, p.kcache, t.box, &t.kmap) && encode_plane(p, p.vcache, t.box, &t.vmap))) t.box = 0;
   auto kernel = attention_tile_kernel<BF16, D>;
   const int smem = TileSmem<D>::kBytes + 1024;  // rounded up to the swizzle's 1024-byte pattern
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<unsigned long long> asked;
+  cudaError_t e = allow_smem(kernel, smem, &asked);
   if (e != cudaSuccess) return e;
   Launch go(dim3(t.n_slots, p.num_kv_heads, t.n_splits), kTileThreads, smem, pdl, stream);
   return cudaLaunchKernelEx(&go.cfg, kernel, t);
@@ -1438,7 +1455,7 @@ cudaError_t launch_typed(const AttentionParams& p, const Plan& plan, bool pdl, i
 long long attention_workspace_bytes(const AttentionParams& p, int sms) {
   const Plan plan = plan_of(p, sms);
   if (plan.slots == 0) return 0;
-  return align256(plan.slots * p.num_heads * 4) + plan.slots * p.num_heads * p.head_dim * 4;
+  return align256(plan.slots * p.num_heads * 4) + align256(plan.slots * p.num_heads * p.head_dim * 4);
 }
 
 cudaError_t launch_attention(const AttentionParams& p, int sms, bool pdl, int* launches, cudaStream_t stream) {

@@ -39,6 +39,11 @@ except AttributeError:  # pragma: no cover - older / newer torch
     _raw_stream = None
 
 
+# The same two lookups for callers that hold a device index (CUDA is initialised by then).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream_of = _raw_stream or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 # Host address of a registered host pool -> the address the GPU uses for the same memory
 # (filled by kv_worker.HostPool; read by the torch custom op of swap_blocks).
 HOST_POOL_DEVICE_PTR: Dict[int, int] = {}

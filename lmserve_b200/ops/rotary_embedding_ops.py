@@ -10,12 +10,13 @@ normalise every query and key head before they rotate it.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple
 
 import torch
 
 from .. import _lib
-from .cache_ops import _OnDevice, _require_cuda, _slots_i64, _stream_ptr
+from .cache_ops import _OnDevice, _current_device, _packer, _raw_stream_of, _require_cuda, _slots_i64, _stream_ptr
 
 _DTYPE_CODE = {torch.float16: 0, torch.bfloat16: 1}
 
@@ -155,63 +156,105 @@ def rotary_pos_emb_and_cache(query: torch.Tensor, key: torch.Tensor, value: torc
     return (q_out, k_out) if return_key else q_out
 
 
-def _check_cache(query, key, value, head_dim, kv_cache, slot_mapping):
-    """Validates the cache side of a fused rotary call; returns the slots."""
-    _require_cuda("value", value)
-    _require_cuda("kv_cache", kv_cache)
-    if value.shape != key.shape or value.dtype != key.dtype or value.stride(1) != 1:
-        raise ValueError("value must match key in shape, dtype and layout")
-    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2 or kv_cache.dtype != key.dtype:
-        raise ValueError("kv_cache must be one layer [num_blocks, 2, block_size, H, D] of the key dtype")
-    NB, _, BS, H, D = kv_cache.shape
-    if D != head_dim or H * D != key.shape[1]:
-        raise ValueError("kv_cache heads do not match key")
-    if NB and kv_cache.stride()[1:] != (BS * H * D, H * D, D, 1):
-        raise ValueError("each cache block must be contiguous")
-    slots = _slots_i64(slot_mapping, query.device)
-    if slots.numel() != query.shape[0]:
-        raise ValueError("slot_mapping must have one entry per token")
-    return slots
+_qk_norm_entry: Optional[int] = None
 
 
-def _qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps,
-             kv_cache, slot_mapping, return_key):
-    _check_inputs(query, key, positions, cos_sin_cache, head_dim)
-    dev, dtype = query.device, query.dtype
+def _refuse_qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cache, head_dim, kv_cache, slots):
+    """Names what is wrong with the arguments of a head norm + rotary call."""
     for n, t in (("query_weight", query_weight), ("key_weight", key_weight)):
         _require_cuda(n, t)
+    _check_inputs(query, key, positions, cos_sin_cache, head_dim)
+    if head_dim <= 0 or not query.shape[1] or not key.shape[1]:
+        raise ValueError("query and key need one head of head_dim elements at least")
+    dev, dtype = query.device, query.dtype
+    for n, t in (("query_weight", query_weight), ("key_weight", key_weight)):
         if t.dtype != dtype or t.shape != (head_dim,) or not t.is_contiguous():
             raise ValueError(f"{n} must be a contiguous [head_dim] vector of the query dtype")
+    if positions.dim() != 1:
+        raise ValueError("positions must be a vector")
+    if kv_cache is not None:
+        _require_cuda("value", value)
+        _require_cuda("kv_cache", kv_cache)
+        if value.shape != key.shape or value.dtype != dtype or value.stride(1) != 1:
+            raise ValueError("value must match key in shape, dtype and layout")
+        if kv_cache.dim() != 5 or kv_cache.shape[1] != 2 or kv_cache.dtype != dtype:
+            raise ValueError("kv_cache must be one layer [num_blocks, 2, block_size, H, D] of the key dtype")
+        NB, _, BS, H, D = kv_cache.shape
+        if D != head_dim or H * D != key.shape[1]:
+            raise ValueError("kv_cache heads do not match key")
+        if NB and kv_cache.stride()[1:] != (BS * H * D, H * D, D, 1):
+            raise ValueError("each cache block must be contiguous")
+        if slots.dim() != 1 or slots.shape[0] != query.shape[0]:
+            raise ValueError("slot_mapping must have one entry per token")
     for n, t in (("key", key), ("positions", positions), ("cos_sin_cache", cos_sin_cache),
                  ("query_weight", query_weight), ("key_weight", key_weight), ("value", value),
                  ("kv_cache", kv_cache)):
         if t is not None and t.device != dev:
             raise ValueError(f"{n} must be on the device of query ({dev}), got {t.device}")
-    slots = None
-    if kv_cache is not None:
-        slots = _check_cache(query, key, value, head_dim, kv_cache, slot_mapping)
-    q_out = torch.empty(query.shape, dtype=dtype, device=dev)
-    k_out = torch.empty(key.shape, dtype=dtype, device=dev) if return_key else None
-    T = query.shape[0]
+    raise ValueError("unsupported arguments of a head norm + rotary call")
+
+
+def _qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps,
+             kv_cache, slot_mapping, return_key):
+    # One such call a layer: attributes are read once, all checks are one expression, and only a
+    # call that fails it is looked at again, to say what is wrong.
+    for t in (query, key, query_weight, key_weight, positions, cos_sin_cache):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"expected a torch.Tensor, got {type(t).__name__}")
+    dtype, idx = query.dtype, query.get_device()
+    code = _DTYPE_CODE.get(dtype)
+    qshape, kshape, cshape = query.shape, key.shape, cos_sin_cache.shape
+    slots = slot_mapping
+    ok = (idx >= 0 and code is not None and len(qshape) == 2 and len(kshape) == 2 and len(cshape) == 2 and head_dim > 0
+          and key.dtype is dtype and cos_sin_cache.dtype is dtype and query_weight.dtype is dtype
+          and key_weight.dtype is dtype and key.get_device() == idx and cos_sin_cache.get_device() == idx
+          and query_weight.get_device() == idx and key_weight.get_device() == idx and positions.get_device() == idx)
+    if ok:
+        T = qshape[0]
+        qstride, kstride, cstride, pdtype = query.stride(), key.stride(), cos_sin_cache.stride(), positions.dtype
+        heads, kv_heads = qshape[1] // head_dim, kshape[1] // head_dim
+        ok = (kshape[0] == T and heads > 0 and kv_heads > 0 and heads * head_dim == qshape[1]
+              and kv_heads * head_dim == kshape[1] and cshape[1] == 2 * head_dim
+              and qstride[1] == 1 and kstride[1] == 1 and cstride[1] == 1
+              and query_weight.shape == key_weight.shape == (head_dim,) and query_weight.is_contiguous()
+              and key_weight.is_contiguous() and positions.shape == (T,)
+              and (pdtype is torch.int32 or pdtype is torch.int64))
+    if ok and kv_cache is not None:
+        lshape, lstride, vstride = kv_cache.shape, kv_cache.stride(), value.stride()
+        row = kv_heads * head_dim
+        if slots.dtype is not torch.int64 or slots.get_device() != idx or not slots.is_contiguous():
+            slots = _slots_i64(slot_mapping, query.device)
+        ok = (len(lshape) == 5 and lshape[1] == 2 and lshape[3] == kv_heads and lshape[4] == head_dim
+              and (lshape[0] == 0 or lstride[1:] == (lshape[2] * row, row, head_dim, 1))
+              and kv_cache.dtype is dtype and value.dtype is dtype and kv_cache.get_device() == idx
+              and value.get_device() == idx and value.shape == kshape and vstride[1] == 1 and slots.shape == (T,))
+    if not ok:
+        _refuse_qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cache, head_dim, kv_cache, slots)
+    q_out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(key, memory_format=torch.contiguous_format) if return_key else None
     if T:
-        es = 2
-        positions = positions.contiguous()
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
+        one = T == 1  # the distance to a next token means nothing
+        words = [query.data_ptr(), key.data_ptr(), None, 0 if one else qstride[0] * 2, 0 if one else kstride[0] * 2, 0,
+                 query_weight.data_ptr(), key_weight.data_ptr(), float(eps), positions.data_ptr(),
+                 1 if pdtype is torch.int64 else 0, cos_sin_cache.data_ptr(), cstride[0] * 2, q_out.data_ptr(),
+                 qshape[1] * 2, k_out.data_ptr() if return_key else None, kshape[1] * 2,
+                 None, None, 0, 0, None, T, heads, kv_heads, head_dim, code, 0, 0, cshape[0]]
         if kv_cache is not None:
-            NB, _, BS, H, D = kv_cache.shape
-            kptr = kv_cache.data_ptr()
-            cache = (kptr, kptr + BS * H * D * es, kv_cache.stride(0) * es, H * D * es, slots.data_ptr())
-            v_ptr, v_tok, bound = value.data_ptr(), value.stride(0) * es, NB * BS
+            base = kv_cache.data_ptr()
+            words[2] = value.data_ptr()
+            words[5] = 0 if one else vstride[0] * 2
+            words[17:22] = base, base + lshape[2] * row * 2, lstride[0] * 2, row * 2, slots.data_ptr()
+            words[27:29] = lshape[2], lshape[0] * lshape[2]
+        global _qk_norm_entry
+        if _qk_norm_entry is None:
+            _qk_norm_entry = ctypes.cast(_lib.lib().lms_qk_norm_rope_and_cache, ctypes.c_void_p).value
+        if idx != _current_device():
+            with torch.cuda.device(idx):
+                rc = _packer.call_words(_qk_norm_entry, _raw_stream_of(idx), words)
         else:
-            cache, v_ptr, v_tok, bound, BS = (None, None, 0, 0, None), None, 0, 0, 0
-        with _OnDevice(dev):
-            rc = _lib.lib().lms_qk_norm_rope_and_cache(
-                query.data_ptr(), key.data_ptr(), v_ptr, query.stride(0) * es, key.stride(0) * es, v_tok,
-                query_weight.data_ptr(), key_weight.data_ptr(), eps, positions.data_ptr(),
-                1 if positions.dtype == torch.int64 else 0, cos_sin_cache.data_ptr(),
-                cos_sin_cache.stride(0) * es, q_out.data_ptr(), q_out.stride(0) * es,
-                k_out.data_ptr() if return_key else None, k_out.stride(0) * es if return_key else 0,
-                *cache, T, query.shape[1] // head_dim, key.shape[1] // head_dim, head_dim,
-                _DTYPE_CODE[dtype], BS, bound, cos_sin_cache.shape[0], _stream_ptr(dev))
+            rc = _packer.call_words(_qk_norm_entry, _raw_stream_of(idx), words)
         if rc:
             _lib.check(rc)
     return (q_out, k_out) if return_key else q_out

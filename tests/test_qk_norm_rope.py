@@ -193,24 +193,27 @@ A = 0x10000  # aligned, never dereferenced
 
 
 def test_argument_errors_of_the_c_entry():
-    f = _lib.lib().lms_qk_norm_rope_and_cache
+    entry = _lib.lib().lms_qk_norm_rope_and_cache
+    assert entry(None, None) == _lib.LMS_ERR_NULL
 
-    def args(**kw):
+    def f(**kw):
         d = dict(q=A, k=A, v=A, qt=2048, kt=512, vt=512, qw=A, kw=A, eps=1e-6, pos=A, p64=0, cs=A, row=512, qo=A,
-                 qot=2048, ko=None, kot=0, kc=A, vc=A, bst=8192, sst=512, slots=A, T=4, nh=8, nkv=2, hd=128, dt=1,
-                 bs=16, ns=64, mp=32, stream=None)
+                 qot=2048, ko=0, kot=0, kc=A, vc=A, bst=8192, sst=512, slots=A, T=4, nh=8, nkv=2, hd=128, dt=1,
+                 bs=16, ns=64, mp=32)
         d.update(kw)
-        return tuple(d.values())
+        words = (ctypes.c_int64 * len(d))(*[int(v or 0) if n != "eps" else 0 for n, v in d.items()])
+        ctypes.cast(ctypes.byref(words, 64), ctypes.POINTER(ctypes.c_double))[0] = d["eps"]
+        return entry(words, None)
 
-    assert f(*args(T=0)) == _lib.LMS_OK
+    assert f(T=0) == _lib.LMS_OK
     for kw in (dict(T=-1), dict(nh=0), dict(dt=2), dict(eps=-1.0), dict(eps=float("nan")), dict(bs=0), dict(mp=-1)):
-        assert f(*args(**kw)) == _lib.LMS_ERR_RANGE, kw
+        assert f(**kw) == _lib.LMS_ERR_RANGE, kw
     for kw in (dict(hd=24), dict(hd=528)):
-        assert f(*args(**kw)) == _lib.LMS_ERR_UNSUPPORTED, kw
+        assert f(**kw) == _lib.LMS_ERR_UNSUPPORTED, kw
     for kw in (dict(q=None), dict(qw=None), dict(cs=None), dict(vc=None), dict(slots=None), dict(v=None)):
-        assert f(*args(**kw)) == _lib.LMS_ERR_NULL, kw
+        assert f(**kw) == _lib.LMS_ERR_NULL, kw
     for kw in (dict(q=A + 8), dict(kw=A + 2), dict(qt=2050), dict(pos=A + 2), dict(slots=A + 4)):
-        assert f(*args(**kw)) == _lib.LMS_ERR_ALIGN, kw
+        assert f(**kw) == _lib.LMS_ERR_ALIGN, kw
 
 
 def test_cpu_tensors_are_refused():
