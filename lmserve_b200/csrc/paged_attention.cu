@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "kernels.cuh"
 
@@ -674,6 +675,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
 constexpr int kRows = 128;       // rows of a tile
 constexpr int kKeys = 128;       // keys of a tile
 constexpr int kTileThreads = 384;
+__device__ constexpr bool kEmulated[8] = {false, false, true, false, false, false, true, false};
 
 struct TileParams {
   CUtensorMap kmap, vmap;
@@ -697,7 +699,7 @@ struct TileSmem {
 
 struct TileBars {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-  uint64_t qfull, sfull[2], pfull[2], ofull[2], done;
+  uint64_t qfull, sfull[2], pfull[2][2], ofull[2], done;
   uint32_t tmem;
   int dead;
 };
@@ -722,6 +724,68 @@ __device__ __forceinline__ void tc_ld32(uint32_t* r, uint32_t addr) {
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
+// Two fp32 lanes in one instruction.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of two values on the FMA pipe, for 2^-126 <= 2^x < 2^127 (smaller ones give 2^-126): n = x
+// rounded to the nearest integer by adding 1.5 * 2^23, whose sum carries n in its low bits, then 2^(x - n)
+// by the polynomial of degree 5 with the smallest relative error on [-1/2, 1/2] (2.1e-7 evaluated in
+// fp32, that of the special-function unit), then n into the exponent.
+__device__ __forceinline__ float2 exp2_poly(uint64_t x) {
+  float2 v = unpack2(x);
+  const uint64_t a = pack2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+  const uint64_t t = add2(a, pack2(12582912.f, 12582912.f));
+  const uint64_t n = add2(t, pack2(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(n, pack2(-1.f, -1.f), a);
+  uint64_t p = pack2(0.001327647129073739f, 0.001327647129073739f);
+  p = fma2(p, f, pack2(0.009675541892647743f, 0.009675541892647743f));
+  p = fma2(p, f, pack2(0.05550713092088699f, 0.05550713092088699f));
+  p = fma2(p, f, pack2(0.24022120237350464f, 0.24022120237350464f));
+  p = fma2(p, f, pack2(0.6931469440460205f, 0.6931469440460205f));
+  p = fma2(p, f, pack2(1.0000001192092896f, 1.0000001192092896f));
+  v = unpack2(p);
+  const float2 e = unpack2(t);
+  return make_float2(__uint_as_float(__float_as_uint(v.x) + (__float_as_uint(e.x) << 23)),
+                     __uint_as_float(__float_as_uint(v.y) + (__float_as_uint(e.y) << 23)));
+}
+__device__ __forceinline__ void tc_ld16(uint32_t* r, uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -734,29 +798,34 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t* r) {
       : "memory");
 }
 
-// Shared memory operand: rows (or K groups) of 128 bytes, 128-byte swizzle, 8-row groups 1024 bytes
-// apart; lbo: bytes between 64-element chunks of an operand whose rows run along K.
-__device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t lbo) {
-  return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
-}
+// Shared memory operand of an MMA: rows (or K groups) of 128 bytes, 128-byte swizzle, 8-row groups
+// 1024 bytes apart.  The low word holds the address and, for an operand whose rows run along K, the
+// distance of its 64-element chunks (lbo); a step along K adds to the low word alone.
+__device__ __forceinline__ uint32_t umma_low(uint32_t addr, uint32_t lbo) { return ((addr & 0x3ffffu) >> 4) | ((lbo >> 4) << 16); }
+constexpr uint32_t kUmmaHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 // kind::f16, fp32 accumulators: element type (0 fp16, 1 bf16), M = 128, N, B along K or along N.
 __device__ __forceinline__ constexpr uint32_t umma_idesc(bool bf16, int n, bool b_along_n) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_along_n ? 1u : 0u) << 16) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// One thread of the warp, the same each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+template <uint32_t IDESC>
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-      "r"(add ? 1u : 0u)
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.b64 x, {%1, %4};\n\tmov.b64 y, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(add), "n"(kUmmaHigh), "n"(IDESC)
       : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+template <uint32_t IDESC>
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
-      "r"(add ? 1u : 0u)
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.b64 y, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %5, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(add), "n"(kUmmaHigh), "n"(IDESC)
       : "memory");
 }
 
@@ -823,7 +892,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   extern __shared__ __align__(1024) char smem_raw[];
   __shared__ TileBars bars;
   const AttentionParams& a = p.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // known to be uniform
   const int G = a.num_heads / a.num_kv_heads;
   const int kvh = blockIdx.y;
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -891,10 +960,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       mbar_init(&bars.vfull[s], 1);
       mbar_init(&bars.vempty[s], 1);
     }
-    mbar_init(&bars.qfull, 2 * kRows);
+    mbar_init(&bars.qfull, 8);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.sfull[i], 1);
-      mbar_init(&bars.pfull[i], kRows);
+      mbar_init(&bars.pfull[i][0], 4);
+      mbar_init(&bars.pfull[i][1], 4);
       mbar_init(&bars.ofull[i], 1);
     }
     mbar_init(&bars.done, 1);
@@ -921,8 +991,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     return __all_sync(0xffffffffu, ok);  // a warp goes on or leaves as one
   };
 
+  // Registers move from the warpgroup of the copies and the MMAs to the two of the softmax, whose
+  // threads hold a row of S: (2 * 216 + 72) * 128 = 384 * 168, what the block was launched with.
   if (warp < 8) {
     // ------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int i = warp >> 2;
     {  // Q row -> shared memory; rows that do not exist are zeros
       const char* src = a.q + (long long)(t_begin + tok) * a.q_tok + (long long)(kvh * G + g) * D * 2;
@@ -937,7 +1010,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                      "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip) : "memory");
       }
       fence_proxy_async();
-      mbar_arrive(&bars.qfull);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.qfull);
     }
     if (i < n_tiles) {
       const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // lane 32 * (warp % 4) in bits 16..
@@ -956,48 +1030,77 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           for (int c = 0; c < kKeys; c += 32) tc_ld32(raw + c, t_s + c);
           tc_wait_ld();
           const int seen = limit - (tile0 + j) * kKeys;
-          if (!__all_sync(0xffffffffu, seen >= kKeys)) {
+          const bool whole = __all_sync(0xffffffffu, seen >= kKeys);  // no key of the tile is masked
+          if (!whole) {
 #pragma unroll
             for (int c = 0; c < kKeys; ++c)
               if (c >= seen) s[c] = -INFINITY;
           }
-          float top = -INFINITY;
+          float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-          for (int c = 0; c < kKeys; ++c) top = fmaxf(top, s[c]);
+          for (int c = 4; c + 8 <= kKeys; c += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tops[e] = max3(tops[e], s[c + e], s[c + 4 + e]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) tops[e] = max3(tops[e], s[kKeys - 4 + e], tops[0]);
+          float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
           top = top == -INFINITY ? top : top * scale2;
           float keep = 1.f;
-          if (top > m + kLazy) {
+          if (!(top <= m + kLazy)) {  // a NaN score, too, moves it: the row is NaN from here on
             keep = exp2_fast(m - top);
             m = top;
           }
-          const bool moved = __any_sync(0xffffffffu, keep != 1.f);
-          const float base = m == -INFINITY ? 0.f : m;
-          float sum = 0.f;
-          uint32_t w[kKeys / 2];
-#pragma unroll
-          for (int c = 0; c < kKeys; c += 2) {
-            const float x = exp2_fast(fmaf(s[c], scale2, -base)), y = exp2_fast(fmaf(s[c + 1], scale2, -base));
-            sum += x + y;
-            w[c / 2] = down2<BF16>(x, y);
-          }
-          l = fmaf(l, keep, sum);
-          tc_st32(t_s, w);
-          tc_st32(t_s + 32, w + 32);
-          if (moved && j > 0) {
+          if (__any_sync(0xffffffffu, keep != 1.f) && j > 0) {
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tc_ld32(o, t_o + c);
+            for (int c = 0; c < D; c += 16) {
+              uint32_t o[16];
+              tc_ld16(o, t_o + c);
               tc_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-              tc_st32(t_o + c, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+              tc_st16(t_o + c, o);
             }
           }
-          tc_wait_st();
+          const float base = m == -INFINITY ? 0.f : m;
+          const uint64_t scale_2 = pack2(scale2, scale2), base_2 = pack2(-base, -base);
+          uint64_t sums[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+          // P goes out in two halves, so that the products of the first run beside the second's
+          // exponentials.  Where no key is masked, 2 of every 8 pairs take the FMA pipe: the
+          // special-function unit alone (16 values a clock) would need as long as the four products.
+          auto weights = [&](auto poly) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              uint32_t w[kKeys / 4];
+#pragma unroll
+              for (int c = 0; c < kKeys / 4; ++c) {
+                const int at = half * (kKeys / 2) + 2 * c;
+                const uint64_t x = fma2(pack2(s[at], s[at + 1]), scale_2, base_2);
+                float2 e;
+                if (decltype(poly)::value && kEmulated[c % 8]) {
+                  e = exp2_poly(x);
+                } else {
+                  e = unpack2(x);
+                  e.x = exp2_fast(e.x);
+                  e.y = exp2_fast(e.y);
+                }
+                sums[c & 1] = add2(sums[c & 1], pack2(e.x, e.y));
+                w[c] = down2<BF16>(e.x, e.y);
+              }
+              tc_st32(t_s + half * 32, w);
+              tc_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bars.pfull[i][half]);
+            }
+          };
+          if (whole) weights(std::true_type{});
+          else weights(std::false_type{});
+          const float2 sum = unpack2(add2(sums[0], sums[1]));
+          l = fmaf(l, keep, sum.x + sum.y);
+        } else if (lane == 0) {
+          mbar_arrive(&bars.pfull[i][0]);
+          mbar_arrive(&bars.pfull[i][1]);
         }
-        tc_fence_before();
-        mbar_arrive(&bars.pfull[i]);
       }
       if (ok && wait(&bars.ofull[i], 0) && live) {
         tc_fence_after();
@@ -1063,7 +1166,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         tc_fence_before();
       }
     }
-  } else if (warp < 10) {
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  }
+  if (warp == 8 || warp == 9) {
     // ------------------------------------------------ K (warp 8) and V (warp 9)
     const bool is_k = warp == 8;
     uint64_t* full = is_k ? bars.kfull : bars.vfull;
@@ -1080,12 +1186,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   } else if (warp == 10) {
     // ------------------------------------------------ MMAs
     constexpr uint32_t id_s = umma_idesc(BF16, kKeys, false), id_o = umma_idesc(BF16, D, true);
+    const bool one = elect_one();
+    const uint32_t q_low = umma_low(sm_q, 16), k_low = umma_low(sm_k, 16), v_low = umma_low(sm_v, kHalf);
     auto qk = [&](int i, int s) {
-      if (lane == 0) {
+      if (one) {
+        const uint32_t a_low = q_low + i * (kRows * D * 2 >> 4), b_low = k_low + s * (S::kStage >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * (kRows * 128) + (k & 3) * 32;
-          umma_ss(tmem + i * 128, umma_desc(sm_q + i * kRows * D * 2 + off, 16), umma_desc(sm_k + s * S::kStage + off, 16), id_s, k > 0);
+          const uint32_t off = ((k >> 2) * (kRows * 128) + (k & 3) * 32) >> 4;
+          umma_ss<id_s>(tmem + i * 128, a_low + off, b_low + off, k > 0);
         }
         tc_commit(&bars.sfull[i]);
       }
@@ -1095,28 +1204,36 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     if (ok) {
       tc_fence_after();
       for (int i = 0; i < n_tiles; ++i) qk(i, 0);
-      if (lane == 0) tc_commit(&bars.kempty[0]);
+      if (one) tc_commit(&bars.kempty[0]);
       for (int j = 0; ok && j < n_kv; ++j) {
         const int s = j % ST, n = (j + 1) % ST;
         if (!(ok = wait(&bars.vfull[s], (j / ST) & 1))) break;
         if (j + 1 < n_kv && !(ok = wait(&bars.kfull[n], ((j + 1) / ST) & 1))) break;
         for (int i = 0; i < n_tiles; ++i) {
-          if (!(ok = wait(&bars.pfull[i], j & 1))) break;
-          tc_fence_after();
-          if (lane == 0) {
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)
-              umma_ts(tmem + 256 + i * 128, tmem + i * 128 + k * 8, umma_desc(sm_v + s * S::kStage + k * 2048, kHalf), id_o, j > 0 || k > 0);
+          for (int half = 0; half < 2; ++half) {
+            if (!(ok = ok && wait(&bars.pfull[i][half], j & 1))) break;
+            tc_fence_after();
+            if (one) {
+              const uint32_t b_low = v_low + s * (S::kStage >> 4);
+#pragma unroll
+              for (int k = half * (kKeys / 32); k < (half + 1) * (kKeys / 32); ++k)
+                umma_ts<id_o>(tmem + 256 + i * 128, tmem + i * 128 + k * 8, b_low + k * (2048 >> 4), k > 0 ? 1u : (uint32_t)j);
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+          if (one) {
             if (j + 1 == n_kv) tc_commit(&bars.ofull[i]);
             if (i + 1 == n_tiles) tc_commit(&bars.vempty[s]);
           }
           __syncwarp();
           if (j + 1 < n_kv) qk(i, n);
         }
-        if (ok && j + 1 < n_kv && lane == 0) tc_commit(&bars.kempty[n]);
+        if (ok && j + 1 < n_kv && one) tc_commit(&bars.kempty[n]);
       }
     }
-    if (lane == 0) tc_commit(&bars.done);
+    if (one) tc_commit(&bars.done);
     __syncwarp();
     wait(&bars.done, 0);
   }
@@ -1237,14 +1354,14 @@ struct Plan {
   long long slots;           // of partials, num_heads rows each
 };
 
-// Splits of the keys so that the row tiles fill the GPU, 512 keys a split at least.
+// Splits of the keys so that the row tiles fill the GPU, a tile of keys each at least.
 int splits_of(long long tokens, long long seqs, long long pages, const AttentionParams& p, int sms) {
   const int G = p.num_heads / p.num_kv_heads;
   long long tiles = (tokens * G + 2 * kRows - 1) / (2 * kRows);
   if (tiles < seqs) tiles = seqs;
   const long long keys = pages * p.block_size / (seqs > 0 ? seqs : 1);
   long long n = sms / (tiles * p.num_kv_heads);
-  if (n > keys / 512) n = keys / 512;
+  if (n > keys / kKeys) n = keys / kKeys;
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 
