@@ -905,30 +905,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   const int slot = p.n_slots - 1 - (int)blockIdx.x;
   const int token0 = token_of(p, 0);
   int seq = 0;
-  {
-    int lo = 0, n = p.n_seq;
-    while (n > 1) {
-      const int step = (n + 31) / 32, at = lo + lane * step;
-      const bool below = lane * step < n && (long long)(token_of(p, at) - token0) * G / (2 * kRows) + at <= slot;
-      const int last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
-      n = min(step, n - last * step);
-      lo += last * step;
-    }
-    seq = lo;
+  for (int n = p.n_seq; n > 1;) {
+    const int step = (n + 31) / 32, at = seq + lane * step;
+    const bool below = lane * step < n && (int)((unsigned)((token_of(p, at) - token0) * G) / (2u * kRows)) + at <= slot;
+    const int last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
+    n = min(step, n - last * step);
+    seq += last * step;
   }
+  const int first_page = p.list.indptr[seq], len = list_keys(p.list, seq, a.block_size);
   const int t_begin = token_of(p, seq), t_end = min(token_of(p, seq + 1), a.num_tokens);
   const int n_new = t_end - t_begin;
-  const long long first_slot = (long long)(t_begin - token0) * G / (2 * kRows) + seq;
-  const long long row0 = (slot - first_slot) * (2 * kRows);
-  const long long n_rows = (long long)n_new * G;
+  const int row0 = (slot - (int)((unsigned)((t_begin - token0) * G) / (2u * kRows)) - seq) * (2 * kRows);
+  const int n_rows = n_new * G;
   if (t_begin < 0 || row0 < 0 || row0 >= n_rows) return;
-  const int rows = (int)min(n_rows - row0, 2ll * kRows);
+  const int rows = min(n_rows - row0, 2 * kRows);
   const int n_tiles = rows > kRows ? 2 : 1;
 
   // keys: to the last one that the last row reads
-  const int len = list_keys(p.list, seq, a.block_size);
   int k_end = len;
-  if (p.causal) k_end = min(len, max(0, len - n_new + (int)((row0 + rows - 1) / G) + 1));
+  if (p.causal) k_end = min(len, max(0, len - n_new + (row0 + rows - 1) / G + 1));
   const int kv_tiles = (k_end + kKeys - 1) / kKeys;
   const int tile0 = (int)((long long)kv_tiles * blockIdx.z / p.n_splits);
   const int n_kv = (int)((long long)kv_tiles * (blockIdx.z + 1) / p.n_splits) - tile0;
@@ -936,7 +931,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   // this thread's row (softmax warps)
   const int r = threadIdx.x;                       // row of the tile pair
   const bool has_row = r < rows && r < 2 * kRows;
-  const int tok = (int)((row0 + r) / G), g = (int)((row0 + r) - (long long)tok * G);
+  const int tok = (row0 + r) / G, g = row0 + r - tok * G;
   const long long out_row = (long long)(t_begin + tok) * a.num_heads + kvh * G + g;  // [token][head]
   const long long part_row = ((long long)(p.slot0 + (int)blockIdx.z) * a.num_tokens) * a.num_heads + out_row;
 
@@ -953,6 +948,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     return;
   }
 
+  // the row of Q, on its way before the barriers are set up; rows that do not exist are zeros
+  uint4 qv[D / 8];
+  if (warp < 8) {
+    const char* src = a.q + (long long)(t_begin + tok) * a.q_tok + (long long)(kvh * G + g) * D * 2;
+#pragma unroll
+    for (int c = 0; c < D / 8; ++c) {
+      qv[c] = make_uint4(0, 0, 0, 0);
+      if (has_row) qv[c] = *reinterpret_cast<const uint4*>(src + c * 16);
+    }
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(&bars.kfull[s], 1);
@@ -980,7 +985,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
   const uint32_t sm_q = smem + S::kQ, sm_k = smem + S::kK, sm_v = smem + S::kV;
-  const int first_page = p.list.indptr[seq];
   // The sign of the scale goes into Q; a scale of 0 must still leave masked scores at -infinity.
   const float scale2 = fmaxf(fabsf(a.scale) * kLog2e, 1.1754944e-38f);
 
@@ -997,18 +1001,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     // ------------------------------------------------ softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int i = warp >> 2;
-    {  // Q row -> shared memory; rows that do not exist are zeros
-      const char* src = a.q + (long long)(t_begin + tok) * a.q_tok + (long long)(kvh * G + g) * D * 2;
+    {
       const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
       const int row = r & (kRows - 1);
       const uint32_t dst = sm_q + i * kRows * D * 2 + row * 128;
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (has_row) v = *reinterpret_cast<const uint4*>(src + c * 16);
+      for (int c = 0; c < D / 8; ++c)
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * (kRows * 128) + (((c & 7) ^ (row & 7)) << 4)),
-                     "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip) : "memory");
-      }
+                     "r"(qv[c].x ^ flip), "r"(qv[c].y ^ flip), "r"(qv[c].z ^ flip), "r"(qv[c].w ^ flip) : "memory");
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.qfull);
@@ -1105,35 +1105,58 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       if (ok && wait(&bars.ofull[i], 0) && live) {
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays
-        char* const dst = a.out + (long long)(t_begin + tok) * a.o_tok + (long long)(kvh * G + g) * D * 2;
+        // O leaves through the shared memory of this tile's Q, which nothing reads any more: a thread
+        // has a row, a store instruction should have whole 128-byte lines.
         float finite = 0.f;
+        const unsigned have = __ballot_sync(0xffffffffu, has_row);
+        const uint32_t stage = sm_q + i * kRows * D * 2 + (warp & 3) * 32 * D * 2;
+        auto emit = [&](auto part) {
+          constexpr bool PART = decltype(part)::value;
+          constexpr int kCols = PART ? D / 2 : D;  // of one pass
+          constexpr int kPassBytes = D * 2;        // of one row: what a row of Q took
+          constexpr int kChunks = kPassBytes / 16, kAtOnce = 32 / kChunks;
+          char* const mine = PART ? reinterpret_cast<char*>(p.part.out + part_row * D)
+                                  : a.out + (long long)(t_begin + tok) * a.o_tok + (long long)(kvh * G + g) * D * 2;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tc_ld32(o, t_o + c);
-          tc_wait_ld();
+          for (int pass = 0; pass < D / kCols; ++pass) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) finite = fmaf(__uint_as_float(o[e]), 0.f, finite);
-          if (!has_row) {
-          } else if (p.slot0 >= 0) {
-            float4* d = reinterpret_cast<float4*>(p.part.out + part_row * D + c);
+            for (int c = 0; c < kCols; c += 32) {
+              uint32_t o[32];
+              tc_ld32(o, t_o + pass * kCols + c);
+              tc_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              d[e] = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
-                                 __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
-          } else {
-            uint4* d = reinterpret_cast<uint4*>(dst + c * 2);
+              for (int e = 0; e < 32; ++e) {
+                finite = fmaf(__uint_as_float(o[e]), 0.f, finite);
+                o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+              }
+              constexpr int kPer = PART ? 4 : 8;  // values of a 16-byte chunk
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t v[4];
+              for (int e = 0; e < 32; e += kPer) {
+                uint32_t v[4];
 #pragma unroll
-              for (int x = 0; x < 4; ++x)
-                v[x] = down2<BF16>(__uint_as_float(o[8 * e + 2 * x]) * inv, __uint_as_float(o[8 * e + 2 * x + 1]) * inv);
-              d[e] = make_uint4(v[0], v[1], v[2], v[3]);
+                for (int x = 0; x < 4; ++x)
+                  v[x] = PART ? o[e + x] : down2<BF16>(__uint_as_float(o[(e + 2 * x) & 31]), __uint_as_float(o[(e + 2 * x + 1) & 31]));
+                const int chunk = (c + e) / kPer;
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * kPassBytes + ((chunk ^ (lane & 7)) << 4)),
+                             "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+              }
             }
+            __syncwarp();
+#pragma unroll 4
+            for (int at = 0; at < 32; at += kAtOnce) {
+              const int row = at + lane / kChunks, chunk = lane % kChunks;
+              uint32_t v[4];
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                           : "r"(stage + row * kPassBytes + ((chunk ^ (row & 7)) << 4)) : "memory");
+              char* const dst = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), row));
+              if (have >> row & 1)
+                *reinterpret_cast<uint4*>(dst + pass * kPassBytes + chunk * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
-        }
+        };
+        if (p.slot0 >= 0) emit(std::true_type{});
+        else emit(std::false_type{});
         if (has_row) {
           const float lse2 = l == 0.f ? -INFINITY : m + log2f(l);
           if (p.slot0 >= 0) p.part.lse[part_row] = lse2;
