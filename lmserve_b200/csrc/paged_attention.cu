@@ -659,6 +659,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
 //   warps 0-3, 4-7   softmax of row tile 0 / 1, one thread a row: S from tensor memory, running
 //                    maximum and sum, P = 2^(S - m) in the element type over S's own columns
 //   warp 8, 9        K / V tiles into two-or-more-stage rings
+//   warp 11          describes the pieces of work (persistent CTAs, a two-deep ring), so that the look-up
+//                    of the next one, and its first K and V tiles, run beside the end of the last
 //   warp 10          issues the MMAs: PV of a tile, then the next QK of the same row tile, so that
 //                    one row tile's softmax runs beside the other's products
 //
@@ -699,9 +701,17 @@ struct TileSmem {
 
 struct TileBars {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-  uint64_t qfull, sfull[2], pfull[2][2], ofull[2], done;
+  uint64_t wfull[2], wempty[2], qfull[2], sfull[2], pfull[2][2], ofull[2], done;
   uint32_t tmem;
-  int dead;
+};
+
+// Two row tiles of one key head against a run of key tiles.
+struct TileWork {
+  int t_begin, n_new;     // tokens of the sequence
+  int row0, rows;         // rows of the pair, counted in the sequence; rows == 0: no more work
+  int len, first_page;    // keys of the sequence, place of its first page in the list
+  int tile0, n_kv;        // key tiles
+  int kvh, split;
 };
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -891,73 +901,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   constexpr int ST = S::kStages, kHalf = kKeys * 128;
   extern __shared__ __align__(1024) char smem_raw[];
   __shared__ TileBars bars;
+  __shared__ TileWork work[2];
   const AttentionParams& a = p.a;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // known to be uniform
   const int G = a.num_heads / a.num_kv_heads;
-  const int kvh = blockIdx.y;
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
 
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
-  // The sequence of this slot: sequence i has the slots from rows(i) / 256 + i on, which leaves it
-  // enough of them without a scan; some stay empty.  Late slots, with the longest causal rows, first.
-  const int slot = p.n_slots - 1 - (int)blockIdx.x;
-  const int token0 = token_of(p, 0);
-  int seq = 0;
-  for (int n = p.n_seq; n > 1;) {
-    const int step = (n + 31) / 32, at = seq + lane * step;
-    const bool below = lane * step < n && (int)((unsigned)((token_of(p, at) - token0) * G) / (2u * kRows)) + at <= slot;
-    const int last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
-    n = min(step, n - last * step);
-    seq += last * step;
-  }
-  const int first_page = p.list.indptr[seq], len = list_keys(p.list, seq, a.block_size);
-  const int t_begin = token_of(p, seq), t_end = min(token_of(p, seq + 1), a.num_tokens);
-  const int n_new = t_end - t_begin;
-  const int row0 = (slot - (int)((unsigned)((t_begin - token0) * G) / (2u * kRows)) - seq) * (2 * kRows);
-  const int n_rows = n_new * G;
-  if (t_begin < 0 || row0 < 0 || row0 >= n_rows) return;
-  const int rows = min(n_rows - row0, 2 * kRows);
-  const int n_tiles = rows > kRows ? 2 : 1;
-
-  // keys: to the last one that the last row reads
-  int k_end = len;
-  if (p.causal) k_end = min(len, max(0, len - n_new + (row0 + rows - 1) / G + 1));
-  const int kv_tiles = (k_end + kKeys - 1) / kKeys;
-  const int tile0 = (int)((long long)kv_tiles * blockIdx.z / p.n_splits);
-  const int n_kv = (int)((long long)kv_tiles * (blockIdx.z + 1) / p.n_splits) - tile0;
-
-  // this thread's row (softmax warps)
-  const int r = threadIdx.x;                       // row of the tile pair
-  const bool has_row = r < rows && r < 2 * kRows;
-  const int tok = (row0 + r) / G, g = row0 + r - tok * G;
-  const long long out_row = (long long)(t_begin + tok) * a.num_heads + kvh * G + g;  // [token][head]
-  const long long part_row = ((long long)(p.slot0 + (int)blockIdx.z) * a.num_tokens) * a.num_heads + out_row;
-
-  if (n_kv <= 0) {  // nothing to read: an empty part, or rows of zeros
-    if (has_row) {
-      if (p.slot0 >= 0) {
-        p.part.lse[part_row] = -INFINITY;
-      } else {
-        char* o = a.out + (long long)(t_begin + tok) * a.o_tok + (long long)(kvh * G + g) * D * 2;
-        for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(o + i * 16) = make_uint4(0, 0, 0, 0);
-        if (a.lse != nullptr) a.lse[out_row] = -INFINITY;
-      }
-    }
-    return;
-  }
-
-  // the row of Q, on its way before the barriers are set up; rows that do not exist are zeros
-  uint4 qv[D / 8];
-  if (warp < 8) {
-    const char* src = a.q + (long long)(t_begin + tok) * a.q_tok + (long long)(kvh * G + g) * D * 2;
-#pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
-      qv[c] = make_uint4(0, 0, 0, 0);
-      if (has_row) qv[c] = *reinterpret_cast<const uint4*>(src + c * 16);
-    }
-  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(&bars.kfull[s], 1);
@@ -965,15 +914,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       mbar_init(&bars.vfull[s], 1);
       mbar_init(&bars.vempty[s], 1);
     }
-    mbar_init(&bars.qfull, 8);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.wfull[i], 1);
+      mbar_init(&bars.wempty[i], 11);
+      mbar_init(&bars.qfull[i], 4);
       mbar_init(&bars.sfull[i], 1);
       mbar_init(&bars.pfull[i][0], 4);
       mbar_init(&bars.pfull[i][1], 4);
       mbar_init(&bars.ofull[i], 1);
     }
     mbar_init(&bars.done, 1);
-    bars.dead = 0;
     mbar_fence_init();
   }
   if (warp == 10) {
@@ -984,6 +934,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
   const uint32_t sm_q = smem + S::kQ, sm_k = smem + S::kK, sm_v = smem + S::kV;
   // The sign of the scale goes into Q; a scale of 0 must still leave masked scores at -infinity.
   const float scale2 = fmaxf(fabsf(a.scale) * kLog2e, 1.1754944e-38f);
@@ -994,6 +947,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     if (!ok) report(a.err, kErrWaitTimeout, kWhereAttention, blockIdx.x, bar - bars.kfull);
     return __all_sync(0xffffffffu, ok);  // a warp goes on or leaves as one
   };
+  // The it-th piece of work, once the scheduler has described it; rows == 0 behind the last one.
+  auto next_work = [&](int it) -> TileWork {
+    TileWork k;
+    k.rows = 0;
+    if (wait(&bars.wfull[it & 1], (it >> 1) & 1)) k = work[it & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars.wempty[it & 1]);
+    return k;
+  };
 
   // Registers move from the warpgroup of the copies and the MMAs to the two of the softmax, whose
   // threads hold a row of S: (2 * 216 + 72) * 128 = 384 * 168, what the block was launched with.
@@ -1001,27 +963,55 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     // ------------------------------------------------ softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int i = warp >> 2;
-    {
-      const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-      const int row = r & (kRows - 1);
-      const uint32_t dst = sm_q + i * kRows * D * 2 + row * 128;
+    const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // lane 32 * (warp % 4) in bits 16..
+    const uint32_t t_s = lanes + i * 128, t_o = lanes + 256 + i * 128;
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+    const int r = threadIdx.x;  // row of the tile pair
+    int tiles = 0, pieces = 0;  // S tiles and pieces of work seen by this row tile
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      const TileWork k = next_work(it);
+      if (k.rows == 0) break;
+      const bool has_row = r < k.rows;
+      const int tok = (k.row0 + r) / G, g = k.row0 + r - tok * G;
+      const long long out_row = (long long)(k.t_begin + tok) * a.num_heads + k.kvh * G + g;  // [token][head]
+      const long long part_row = ((long long)(p.slot0 + k.split) * a.num_tokens) * a.num_heads + out_row;
+      if (k.n_kv == 0) {  // nothing to read: an empty part, or rows of zeros
+        if (has_row) {
+          if (p.slot0 >= 0) {
+            p.part.lse[part_row] = -INFINITY;
+          } else {
+            char* o = a.out + (long long)(k.t_begin + tok) * a.o_tok + (long long)(k.kvh * G + g) * D * 2;
+            for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(o + c * 16) = make_uint4(0, 0, 0, 0);
+            if (a.lse != nullptr) a.lse[out_row] = -INFINITY;
+          }
+        }
+        continue;
+      }
+      if (i * kRows >= k.rows) continue;  // one row tile only
+      {  // the row of Q; rows that do not exist are zeros
+        const char* src = a.q + (long long)(k.t_begin + tok) * a.q_tok + (long long)(k.kvh * G + g) * D * 2;
+        uint4 qv[D / 8];
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * (kRows * 128) + (((c & 7) ^ (row & 7)) << 4)),
-                     "r"(qv[c].x ^ flip), "r"(qv[c].y ^ flip), "r"(qv[c].z ^ flip), "r"(qv[c].w ^ flip) : "memory");
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.qfull);
-    }
-    if (i < n_tiles) {
-      const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // lane 32 * (warp % 4) in bits 16..
-      const uint32_t t_s = lanes + i * 128, t_o = lanes + 256 + i * 128;
-      const bool live = (r & ~31) < rows;  // the warp has a row
-      const int limit = p.causal ? min(len, len - n_new + tok + 1) : len;  // keys below it are read
+        for (int c = 0; c < D / 8; ++c) {
+          qv[c] = make_uint4(0, 0, 0, 0);
+          if (has_row) qv[c] = *reinterpret_cast<const uint4*>(src + c * 16);
+        }
+        const int row = r & (kRows - 1);
+        const uint32_t dst = sm_q + i * kRows * D * 2 + row * 128;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * (kRows * 128) + (((c & 7) ^ (row & 7)) << 4)),
+                       "r"(qv[c].x ^ flip), "r"(qv[c].y ^ flip), "r"(qv[c].z ^ flip), "r"(qv[c].w ^ flip) : "memory");
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.qfull[i]);
+      }
+      const bool live = (r & ~31) < k.rows;  // the warp has a row
+      const int limit = p.causal ? min(k.len, k.len - k.n_new + tok + 1) : k.len;  // keys below it are read
       float m = -INFINITY, l = 0.f;
-      bool ok = true;
-      for (int j = 0; j < n_kv; ++j) {
-        if (!(ok = wait(&bars.sfull[i], j & 1))) break;
+      for (int j = 0; j < k.n_kv; ++j, ++tiles) {
+        if (!(ok = wait(&bars.sfull[i], tiles & 1))) break;
         tc_fence_after();
         if (live) {
           float s[kKeys];
@@ -1029,7 +1019,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
 #pragma unroll
           for (int c = 0; c < kKeys; c += 32) tc_ld32(raw + c, t_s + c);
           tc_wait_ld();
-          const int seen = limit - (tile0 + j) * kKeys;
+          const int seen = limit - (k.tile0 + j) * kKeys;
           const bool whole = __all_sync(0xffffffffu, seen >= kKeys);  // no key of the tile is masked
           if (!whole) {
 #pragma unroll
@@ -1102,21 +1092,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           mbar_arrive(&bars.pfull[i][1]);
         }
       }
-      if (ok && wait(&bars.ofull[i], 0) && live) {
+      if (ok) ok = wait(&bars.ofull[i], pieces & 1);
+      ++pieces;
+      if (ok && live) {
         tc_fence_after();
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays
-        // O leaves through the shared memory of this tile's Q, which nothing reads any more: a thread
-        // has a row, a store instruction should have whole 128-byte lines.
+        // O leaves through the shared memory of the warp's own Q rows, which nothing reads any more: a
+        // thread has a row, a store instruction should have whole 128-byte lines.
         float finite = 0.f;
         const unsigned have = __ballot_sync(0xffffffffu, has_row);
-        const uint32_t stage = sm_q + i * kRows * D * 2 + (warp & 3) * 32 * D * 2;
+        const uint32_t stage = sm_q + i * kRows * D * 2 + (warp & 3) * 32 * 128;
         auto emit = [&](auto part) {
           constexpr bool PART = decltype(part)::value;
           constexpr int kCols = PART ? D / 2 : D;  // of one pass
           constexpr int kPassBytes = D * 2;        // of one row: what a row of Q took
           constexpr int kChunks = kPassBytes / 16, kAtOnce = 32 / kChunks;
           char* const mine = PART ? reinterpret_cast<char*>(p.part.out + part_row * D)
-                                  : a.out + (long long)(t_begin + tok) * a.o_tok + (long long)(kvh * G + g) * D * 2;
+                                  : a.out + (long long)(k.t_begin + tok) * a.o_tok + (long long)(k.kvh * G + g) * D * 2;
 #pragma unroll 1
           for (int pass = 0; pass < D / kCols; ++pass) {
 #pragma unroll
@@ -1137,7 +1129,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 for (int x = 0; x < 4; ++x)
                   v[x] = PART ? o[e + x] : down2<BF16>(__uint_as_float(o[(e + 2 * x) & 31]), __uint_as_float(o[(e + 2 * x + 1) & 31]));
                 const int chunk = (c + e) / kPer;
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * kPassBytes + ((chunk ^ (lane & 7)) << 4)),
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + (chunk >> 3) * (kRows * 128) + lane * 128 + (((chunk & 7) ^ (lane & 7)) << 4)),
                              "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
               }
             }
@@ -1147,7 +1139,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
               const int row = at + lane / kChunks, chunk = lane % kChunks;
               uint32_t v[4];
               asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                           : "r"(stage + row * kPassBytes + ((chunk ^ (row & 7)) << 4)) : "memory");
+                           : "r"(stage + (chunk >> 3) * (kRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) : "memory");
               char* const dst = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), row));
               if (have >> row & 1)
                 *reinterpret_cast<uint4*>(dst + pass * kPassBytes + chunk * 16) = make_uint4(v[0], v[1], v[2], v[3]);
@@ -1170,13 +1162,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           const int who = __ffs(again) - 1;
           again &= again - 1;
           const int w_tok = __shfl_sync(0xffffffffu, tok, who), w_g = __shfl_sync(0xffffffffu, g, who);
-          const int w_end = min(__shfl_sync(0xffffffffu, limit, who), (tile0 + n_kv) * kKeys);
+          const int w_end = min(__shfl_sync(0xffffffffu, limit, who), (k.tile0 + k.n_kv) * kKeys);
           const long long w_part = __shfl_sync(0xffffffffu, part_row, who), w_out = __shfl_sync(0xffffffffu, out_row, who);
-          const long long head = (long long)(kvh * G + w_g) * D * 2;
-          RowWalk<BF16, D / 64> walk(a.q + (long long)(t_begin + w_tok) * a.q_tok + head, D, lane);
-          walk.walk(a, p.list, first_page, kvh, tile0 * kKeys, w_end, lane);
+          const long long head = (long long)(k.kvh * G + w_g) * D * 2;
+          RowWalk<BF16, D / 64> walk(a.q + (long long)(k.t_begin + w_tok) * a.q_tok + head, D, lane);
+          walk.walk(a, p.list, k.first_page, k.kvh, k.tile0 * kKeys, w_end, lane);
           if (p.slot0 < 0) {
-            walk.store(a.out + (long long)(t_begin + w_tok) * a.o_tok + head, D, lane);
+            walk.store(a.out + (long long)(k.t_begin + w_tok) * a.o_tok + head, D, lane);
             if (a.lse != nullptr && lane == 0) a.lse[w_out] = walk.lse2() * kLn2;
           } else {
 #pragma unroll
@@ -1197,15 +1189,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     const bool is_k = warp == 8;
     uint64_t* full = is_k ? bars.kfull : bars.vfull;
     uint64_t* empty = is_k ? bars.kempty : bars.vempty;
-    int j = 0;
-    for (; j < n_kv; ++j) {
-      const int s = j % ST, use = j / ST;
-      if (use > 0 && !wait(&empty[s], (use - 1) & 1)) break;
-      load_tile<D>(p, is_k ? &p.kmap : &p.vmap, is_k ? a.kcache : a.vcache, kvh, first_page, len, tile0 + j,
-                   (is_k ? sm_k : sm_v) + s * S::kStage, &full[s], lane);
+    int n = 0;  // tiles loaded so far
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      const TileWork k = next_work(it);
+      if (k.rows == 0) break;
+      for (int j = 0; j < k.n_kv; ++j, ++n) {
+        const int s = n % ST, use = n / ST;
+        if (use > 0 && !(ok = wait(&empty[s], (use - 1) & 1))) break;
+        load_tile<D>(p, is_k ? &p.kmap : &p.vmap, is_k ? a.kcache : a.vcache, k.kvh, k.first_page, k.len, k.tile0 + j,
+                     (is_k ? sm_k : sm_v) + s * S::kStage, &full[s], lane);
+      }
     }
     // no copy may be in flight when the CTA leaves, whatever the others did
-    for (int d = max(0, j - ST); d < j; ++d) wait(&full[d % ST], (d / ST) & 1);
+    for (int d = max(0, n - ST); d < n; ++d) wait(&full[d % ST], (d / ST) & 1);
   } else if (warp == 10) {
     // ------------------------------------------------ MMAs
     constexpr uint32_t id_s = umma_idesc(BF16, kKeys, false), id_o = umma_idesc(BF16, D, true);
@@ -1223,42 +1220,104 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       }
       __syncwarp();
     };
-    bool ok = wait(&bars.qfull, 0) && wait(&bars.kfull[0], 0);
-    if (ok) {
-      tc_fence_after();
-      for (int i = 0; i < n_tiles; ++i) qk(i, 0);
-      if (one) tc_commit(&bars.kempty[0]);
-      for (int j = 0; ok && j < n_kv; ++j) {
-        const int s = j % ST, n = (j + 1) % ST;
-        if (!(ok = wait(&bars.vfull[s], (j / ST) & 1))) break;
-        if (j + 1 < n_kv && !(ok = wait(&bars.kfull[n], ((j + 1) / ST) & 1))) break;
-        for (int i = 0; i < n_tiles; ++i) {
+    int n = 0;                          // tiles so far, both rings
+    int pieces[2] = {0, 0}, tiles[2] = {0, 0};  // of each row tile
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      const TileWork k = next_work(it);
+      if (k.rows == 0) break;
+      if (k.n_kv == 0) continue;
+      const int n_tiles = k.rows > kRows ? 2 : 1;
+      ok = wait(&bars.kfull[n % ST], (n / ST) & 1);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i >= n_tiles || !ok) continue;
+        // a row tile's Q also says that its last S and O have been read
+        ok = wait(&bars.qfull[i], pieces[i]++ & 1);
+        tc_fence_after();
+        if (ok) qk(i, n % ST);
+      }
+      if (ok && one) tc_commit(&bars.kempty[n % ST]);
+      for (int j = 0; ok && j < k.n_kv; ++j, ++n) {
+        const int s = n % ST, next = (n + 1) % ST;
+        if (!(ok = wait(&bars.vfull[s], (n / ST) & 1))) break;
+        if (j + 1 < k.n_kv && !(ok = wait(&bars.kfull[next], ((n + 1) / ST) & 1))) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (i >= n_tiles || !ok) continue;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            if (!(ok = ok && wait(&bars.pfull[i][half], j & 1))) break;
+            ok = ok && wait(&bars.pfull[i][half], tiles[i] & 1);
             tc_fence_after();
-            if (one) {
+            if (ok && one) {
               const uint32_t b_low = v_low + s * (S::kStage >> 4);
 #pragma unroll
-              for (int k = half * (kKeys / 32); k < (half + 1) * (kKeys / 32); ++k)
-                umma_ts<id_o>(tmem + 256 + i * 128, tmem + i * 128 + k * 8, b_low + k * (2048 >> 4), k > 0 ? 1u : (uint32_t)j);
+              for (int c = half * (kKeys / 32); c < (half + 1) * (kKeys / 32); ++c)
+                umma_ts<id_o>(tmem + 256 + i * 128, tmem + i * 128 + c * 8, b_low + c * (2048 >> 4), c > 0 ? 1u : (uint32_t)j);
             }
             __syncwarp();
           }
-          if (!ok) break;
-          if (one) {
-            if (j + 1 == n_kv) tc_commit(&bars.ofull[i]);
+          ++tiles[i];
+          if (ok && one) {
+            if (j + 1 == k.n_kv) tc_commit(&bars.ofull[i]);
             if (i + 1 == n_tiles) tc_commit(&bars.vempty[s]);
           }
           __syncwarp();
-          if (j + 1 < n_kv) qk(i, n);
+          if (ok && j + 1 < k.n_kv) qk(i, next);
         }
-        if (ok && j + 1 < n_kv && one) tc_commit(&bars.kempty[n]);
+        if (ok && j + 1 < k.n_kv && one) tc_commit(&bars.kempty[next]);
       }
     }
     if (one) tc_commit(&bars.done);
     __syncwarp();
     wait(&bars.done, 0);
+  } else if (warp == 11) {
+    // ------------------------------------------------ what to do: pieces blockIdx.x, + gridDim.x, ...
+    const int token0 = token_of(p, 0);
+    int it = 0;
+    bool ok = true;
+    auto tell = [&](const TileWork& k) {
+      if (it >= 2) ok = wait(&bars.wempty[it & 1], ((it >> 1) - 1) & 1);
+      if (ok && lane == 0) {
+        work[it & 1] = k;
+        mbar_arrive(&bars.wfull[it & 1]);
+      }
+      __syncwarp();
+      ++it;
+    };
+    const int per_slot = a.num_kv_heads * p.n_splits;
+    for (long long e = blockIdx.x; ok && e < (long long)p.n_slots * per_slot; e += gridDim.x) {
+      // The sequence of a slot: sequence i has the slots from rows(i) / 256 + i on, which leaves it
+      // enough of them without a scan; some stay empty.  Late slots, with the longest causal rows, first.
+      const int slot = p.n_slots - 1 - (int)(e / per_slot), in_slot = (int)(e % per_slot);
+      int seq = 0;
+      for (int n = p.n_seq; n > 1;) {
+        const int step = (n + 31) / 32, at = seq + lane * step;
+        const bool below = lane * step < n && (int)((unsigned)((token_of(p, at) - token0) * G) / (2u * kRows)) + at <= slot;
+        const int last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
+        n = min(step, n - last * step);
+        seq += last * step;
+      }
+      TileWork k;
+      k.first_page = p.list.indptr[seq];
+      k.len = list_keys(p.list, seq, a.block_size);
+      k.t_begin = token_of(p, seq);
+      k.n_new = min(token_of(p, seq + 1), a.num_tokens) - k.t_begin;
+      k.row0 = (slot - (int)((unsigned)((k.t_begin - token0) * G) / (2u * kRows)) - seq) * (2 * kRows);
+      if (k.t_begin < 0 || k.row0 < 0 || k.row0 >= k.n_new * G) continue;
+      k.rows = min(k.n_new * G - k.row0, 2 * kRows);
+      k.kvh = in_slot % a.num_kv_heads;
+      k.split = in_slot / a.num_kv_heads;
+      // keys: to the last one that the last row reads
+      int k_end = k.len;
+      if (p.causal) k_end = min(k.len, max(0, k.len - k.n_new + (k.row0 + k.rows - 1) / G + 1));
+      const long long kv_tiles = (k_end + kKeys - 1) / kKeys;
+      k.tile0 = (int)(kv_tiles * k.split / p.n_splits);
+      k.n_kv = (int)(kv_tiles * (k.split + 1) / p.n_splits) - k.tile0;
+      tell(k);
+    }
+    TileWork end = {};
+    if (ok) tell(end);
   }
   tc_fence_before();
   __syncthreads();
@@ -1507,7 +1566,7 @@ cudaError_t launch_decode(const AttentionParams& p, const Plan& plan, bool pdl, 
 }
 
 template <bool BF16, int D>
-cudaError_t launch_tile(const AttentionParams& p, const Plan& plan, bool shared, bool pdl, cudaStream_t stream) {
+cudaError_t launch_tile(const AttentionParams& p, const Plan& plan, bool shared, int sms, bool pdl, cudaStream_t stream) {
   TileParams t{};
   t.a = p;
   t.list = shared ? p.prefix : p.own;
@@ -1530,7 +1589,8 @@ cudaError_t launch_tile(const AttentionParams& p, const Plan& plan, bool shared,
   static std::atomic<unsigned long long> asked;
   cudaError_t e = allow_smem(kernel, smem, &asked);
   if (e != cudaSuccess) return e;
-  Launch go(dim3(t.n_slots, p.num_kv_heads, t.n_splits), kTileThreads, smem, pdl, stream);
+  const long long pieces = slots * p.num_kv_heads * t.n_splits;
+  Launch go(dim3((unsigned)(pieces < sms ? pieces : sms)), kTileThreads, smem, pdl, stream);
   return cudaLaunchKernelEx(&go.cfg, kernel, t);
 }
 
@@ -1558,10 +1618,10 @@ cudaError_t launch_rows(const AttentionParams& p, bool pdl, cudaStream_t stream)
 }
 
 template <bool BF16, int D>
-cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, bool pdl, int* launches, cudaStream_t stream) {
+cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, int sms, bool pdl, int* launches, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
   if (plan.shared_splits > 0) {
-    e = launch_tile<BF16, D>(p, plan, true, pdl, stream);
+    e = launch_tile<BF16, D>(p, plan, true, sms, pdl, stream);
     *launches += e == cudaSuccess;
   }
   if (e == cudaSuccess && plan.runs) {
@@ -1570,7 +1630,7 @@ cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, bool pdl, 
     e = few ? launch_decode<BF16, D, 1, kDeep>(p, plan, pdl, stream) : launch_decode<BF16, D, 2, D == 64 ? 5 : 2>(p, plan, pdl, stream);
     *launches += e == cudaSuccess;
   } else if (e == cudaSuccess) {
-    e = launch_tile<BF16, D>(p, plan, false, pdl, stream);
+    e = launch_tile<BF16, D>(p, plan, false, sms, pdl, stream);
     *launches += e == cudaSuccess;
   }
   if (e == cudaSuccess && plan.join) {
@@ -1581,13 +1641,13 @@ cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, bool pdl, 
 }
 
 template <bool BF16>
-cudaError_t launch_typed(const AttentionParams& p, const Plan& plan, bool pdl, int* launches, cudaStream_t stream) {
+cudaError_t launch_typed(const AttentionParams& p, const Plan& plan, int sms, bool pdl, int* launches, cudaStream_t stream) {
   if (plan.rows) {
     *launches = 1;
     return launch_rows<BF16>(p, pdl, stream);
   }
-  return p.head_dim == 64 ? launch_matrix<BF16, 64>(p, plan, pdl, launches, stream)
-                          : launch_matrix<BF16, 128>(p, plan, pdl, launches, stream);
+  return p.head_dim == 64 ? launch_matrix<BF16, 64>(p, plan, sms, pdl, launches, stream)
+                          : launch_matrix<BF16, 128>(p, plan, sms, pdl, launches, stream);
 }
 
 }  // namespace
@@ -1601,8 +1661,8 @@ long long attention_workspace_bytes(const AttentionParams& p, int sms) {
 cudaError_t launch_attention(const AttentionParams& p, int sms, bool pdl, int* launches, cudaStream_t stream) {
   const Plan plan = plan_of(p, sms);
   *launches = 0;
-  return p.is_bf16 ? launch_typed<true>(p, plan, pdl, launches, stream)
-                   : launch_typed<false>(p, plan, pdl, launches, stream);
+  return p.is_bf16 ? launch_typed<true>(p, plan, sms, pdl, launches, stream)
+                   : launch_typed<false>(p, plan, sms, pdl, launches, stream);
 }
 
 }  // namespace lms
