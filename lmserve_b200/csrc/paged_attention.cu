@@ -701,7 +701,7 @@ struct TileSmem {
 
 struct TileBars {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-  uint64_t wfull[2], wempty[2], qfull[2], sfull[2], pfull[2][2], ofull[2], done;
+  uint64_t wfull[2], wempty[2], qfull[2], sfull[2], pfull[2][2], ofull[2], want, grant, done;
   uint32_t tmem;
 };
 
@@ -902,6 +902,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   extern __shared__ __align__(1024) char smem_raw[];
   __shared__ TileBars bars;
   __shared__ TileWork work[2];
+  __shared__ __align__(16) uint4 granted;  // the launch control's answer
   const AttentionParams& a = p.a;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // known to be uniform
   const int G = a.num_heads / a.num_kv_heads;
@@ -923,6 +924,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       mbar_init(&bars.pfull[i][1], 4);
       mbar_init(&bars.ofull[i], 1);
     }
+    mbar_init(&bars.want, 1);
+    mbar_init(&bars.grant, 1);
     mbar_init(&bars.done, 1);
     mbar_fence_init();
   }
@@ -1200,6 +1203,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         load_tile<D>(p, is_k ? &p.kmap : &p.vmap, is_k ? a.kcache : a.vcache, k.kvh, k.first_page, k.len, k.tile0 + j,
                      (is_k ? sm_k : sm_v) + s * S::kStage, &full[s], lane);
       }
+      if (is_k && lane == 0) mbar_arrive(&bars.want);  // time to look for more
     }
     // no copy may be in flight when the CTA leaves, whatever the others did
     for (int d = max(0, n - ST); d < n; ++d) wait(&full[d % ST], (d / ST) & 1);
@@ -1272,7 +1276,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     __syncwarp();
     wait(&bars.done, 0);
   } else if (warp == 11) {
-    // ------------------------------------------------ what to do: pieces blockIdx.x, + gridDim.x, ...
+    // ------------------------------------------------ what to do
+    // The grid has a block for every piece of work.  A resident CTA does its own and then takes over
+    // blocks that have not started (cluster launch control), when the last tile of a piece is on its
+    // way: no counter in memory, and pieces of any length spread evenly.
     const int token0 = token_of(p, 0);
     int it = 0;
     bool ok = true;
@@ -1286,10 +1293,27 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       ++it;
     };
     const int per_slot = a.num_kv_heads * p.n_splits;
-    for (long long e = blockIdx.x; ok && e < (long long)p.n_slots * per_slot; e += gridDim.x) {
+    unsigned e = blockIdx.x;
+    for (int asked = 0; ok; ++asked) {
+      if (asked > 0) {
+        if (lane == 0) {
+          mbar_expect_tx(&bars.grant, 16);
+          asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(&granted)),
+                       "r"(smem_u32(&bars.grant)) : "memory");
+        }
+        if (!(ok = wait(&bars.grant, (asked - 1) & 1))) break;
+        unsigned given;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b128 x;\n\tld.shared.b128 x, [%2];\n\t"
+            "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, x;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+            "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, x;\n\t}" : "=r"(given), "=r"(e) : "r"(smem_u32(&granted)) : "memory");
+        fence_proxy_async();  // read before the next answer is written there
+        __syncwarp();
+        if (given == 0) break;  // every block has been started by now
+      }
       // The sequence of a slot: sequence i has the slots from rows(i) / 256 + i on, which leaves it
       // enough of them without a scan; some stay empty.  Late slots, with the longest causal rows, first.
-      const int slot = p.n_slots - 1 - (int)(e / per_slot), in_slot = (int)(e % per_slot);
+      const int slot = p.n_slots - 1 - (int)(e / (unsigned)per_slot), in_slot = (int)(e % (unsigned)per_slot);
       int seq = 0;
       for (int n = p.n_seq; n > 1;) {
         const int step = (n + 31) / 32, at = seq + lane * step;
@@ -1315,6 +1339,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       k.tile0 = (int)(kv_tiles * k.split / p.n_splits);
       k.n_kv = (int)(kv_tiles * (k.split + 1) / p.n_splits) - k.tile0;
       tell(k);
+      if (ok) ok = wait(&bars.want, (it - 1) & 1);
     }
     TileWork end = {};
     if (ok) tell(end);
@@ -1566,7 +1591,7 @@ cudaError_t launch_decode(const AttentionParams& p, const Plan& plan, bool pdl, 
 }
 
 template <bool BF16, int D>
-cudaError_t launch_tile(const AttentionParams& p, const Plan& plan, bool shared, int sms, bool pdl, cudaStream_t stream) {
+cudaError_t launch_tile(const AttentionParams& p, const Plan& plan, bool shared, bool pdl, cudaStream_t stream) {
   TileParams t{};
   t.a = p;
   t.list = shared ? p.prefix : p.own;
@@ -1590,7 +1615,8 @@ cudaError_t launch_tile(const AttentionParams& p, const Plan& plan, bool shared,
   cudaError_t e = allow_smem(kernel, smem, &asked);
   if (e != cudaSuccess) return e;
   const long long pieces = slots * p.num_kv_heads * t.n_splits;
-  Launch go(dim3((unsigned)(pieces < sms ? pieces : sms)), kTileThreads, smem, pdl, stream);
+  if (pieces > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  Launch go(dim3((unsigned)pieces), kTileThreads, smem, pdl, stream);
   return cudaLaunchKernelEx(&go.cfg, kernel, t);
 }
 
@@ -1618,10 +1644,10 @@ cudaError_t launch_rows(const AttentionParams& p, bool pdl, cudaStream_t stream)
 }
 
 template <bool BF16, int D>
-cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, int sms, bool pdl, int* launches, cudaStream_t stream) {
+cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, bool pdl, int* launches, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
   if (plan.shared_splits > 0) {
-    e = launch_tile<BF16, D>(p, plan, true, sms, pdl, stream);
+    e = launch_tile<BF16, D>(p, plan, true, pdl, stream);
     *launches += e == cudaSuccess;
   }
   if (e == cudaSuccess && plan.runs) {
@@ -1630,7 +1656,7 @@ cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, int sms, b
     e = few ? launch_decode<BF16, D, 1, kDeep>(p, plan, pdl, stream) : launch_decode<BF16, D, 2, D == 64 ? 5 : 2>(p, plan, pdl, stream);
     *launches += e == cudaSuccess;
   } else if (e == cudaSuccess) {
-    e = launch_tile<BF16, D>(p, plan, false, sms, pdl, stream);
+    e = launch_tile<BF16, D>(p, plan, false, pdl, stream);
     *launches += e == cudaSuccess;
   }
   if (e == cudaSuccess && plan.join) {
@@ -1641,13 +1667,13 @@ cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, int sms, b
 }
 
 template <bool BF16>
-cudaError_t launch_typed(const AttentionParams& p, const Plan& plan, int sms, bool pdl, int* launches, cudaStream_t stream) {
+cudaError_t launch_typed(const AttentionParams& p, const Plan& plan, bool pdl, int* launches, cudaStream_t stream) {
   if (plan.rows) {
     *launches = 1;
     return launch_rows<BF16>(p, pdl, stream);
   }
-  return p.head_dim == 64 ? launch_matrix<BF16, 64>(p, plan, sms, pdl, launches, stream)
-                          : launch_matrix<BF16, 128>(p, plan, sms, pdl, launches, stream);
+  return p.head_dim == 64 ? launch_matrix<BF16, 64>(p, plan, pdl, launches, stream)
+                          : launch_matrix<BF16, 128>(p, plan, pdl, launches, stream);
 }
 
 }  // namespace
@@ -1661,8 +1687,8 @@ long long attention_workspace_bytes(const AttentionParams& p, int sms) {
 cudaError_t launch_attention(const AttentionParams& p, int sms, bool pdl, int* launches, cudaStream_t stream) {
   const Plan plan = plan_of(p, sms);
   *launches = 0;
-  return p.is_bf16 ? launch_typed<true>(p, plan, sms, pdl, launches, stream)
-                   : launch_typed<false>(p, plan, sms, pdl, launches, stream);
+  return p.is_bf16 ? launch_typed<true>(p, plan, pdl, launches, stream)
+                   : launch_typed<false>(p, plan, pdl, launches, stream);
 }
 
 }  // namespace lms
