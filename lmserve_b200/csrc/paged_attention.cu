@@ -220,13 +220,14 @@ struct Partials {
 // finished there; one cut by a border leaves a partial in each run (slot 2x if it began in an
 // earlier run, else 2x + 1) for the join kernel.
 //
-// Inside a CTA a warp works alone: head hs = w % HB of the block, every KS-th 16-key tile of the
-// run (KS = 8 / HB), its own ring of stages filled by TMA (a box a page, 128-byte swizzled) or, for
-// page sizes a 16-key box does not fit, by cp.async rows; no block-wide barrier in the loop.  Both
+// Inside a CTA a warp works alone: head hs = w % HB of the block, the ks-th of KS = 8 / HB equal parts
+// of the run, its own ring of stages filled by TMA (a box a page, 128-byte swizzled) or, for page
+// sizes a 16-key box does not fit, by cp.async rows; no barrier in the loop.  Both
 // products are taken transposed, S^T = K Q^T and O^T += V^T P^T (m16n8k16), so that the 16-wide
 // side is full of keys or head elements and the 8-wide side holds the G rows: half the products and
 // registers of the other way round for G <= 8.  S^T turns into the second product's operand with
-// movmatrix.  The KS warps of a head join their (m, l, O) through shared memory when a request ends.
+// movmatrix.  What the borders between the KS parts cut is joined through shared memory at the end
+// (one barrier a CTA; a barrier a request, with the tiles dealt out in turn, cost 2 to 4 us each).
 constexpr int kDecodeWarps = 8;
 constexpr int kTile = 16;  // keys
 
@@ -245,8 +246,17 @@ struct DecodeParams {
 struct __align__(16) TileMeta {
   int request;  // -1: behind the last tile
   int keys;     // keys of the tile that exist
-  int flags;    // 1: first tile of the request in this warp, 2: last
+  int flags;    // 1: first tile of the request in this warp, 2: last, kHead / kTail, kBefore / kBehind
   int slot;     // where the result goes: -1 = the output row (a slot is num_heads rows)
+};
+enum {
+  kHead = 4,    // began in an earlier part of the run (or before it): joined at the end
+  kTail = 8,    // began here and goes on in a later part
+  kBefore = 16, // began before the CTA's run
+  kBehind = 32  // goes on behind the CTA's run
+};
+struct Piece {  // what a warp leaves for the join: its head and its tail
+  int request, flags;
 };
 
 template <int D, int NST>
@@ -255,9 +265,9 @@ struct DecodeSmem {
   static constexpr int kPlane = D / 64 * kHalf;
   static constexpr int kStage = 2 * kPlane;
   static constexpr int kRing = kDecodeWarps * NST * kStage;
-  static constexpr int kMeta = kDecodeWarps * NST * (int)(sizeof(TileMeta) + sizeof(uint64_t));
+  static constexpr int kMeta = kDecodeWarps * (NST * (int)(sizeof(TileMeta) + sizeof(uint64_t)) + 2 * (int)sizeof(Piece));
   static int bytes(int G, int hb) {
-    const int join = hb < kDecodeWarps ? kDecodeWarps * G * (D + 2) * 4 : 0;
+    const int join = hb < kDecodeWarps ? kDecodeWarps * G * (D + 4) * 4 : 0;
     return 1024 + kRing + kMeta + join;
   }
 };
@@ -284,20 +294,23 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
   const uint32_t ring = smem_u32(smem) + warp * NST * S::kStage;
   TileMeta* const meta = reinterpret_cast<TileMeta*>(smem + S::kRing) + warp * NST;
   uint64_t* const full = reinterpret_cast<uint64_t*>(smem + S::kRing + kDecodeWarps * NST * sizeof(TileMeta)) + warp * NST;
-  float* const joins = reinterpret_cast<float*>(smem + S::kRing + S::kMeta);
+  Piece* const pieces = reinterpret_cast<Piece*>(smem + S::kRing + kDecodeWarps * NST * (sizeof(TileMeta) + sizeof(uint64_t)));
+  // [warp][G][D] heads, then [warp][G] their maxima and sums; a tail takes the warp's own ring
+  float* const heads = reinterpret_cast<float*>(smem + S::kRing + S::kMeta);
 
   if (TMA && lane < NST) mbar_init(&full[lane], 1);  // the warp's own
+  if (lane < 2) pieces[warp * 2 + lane] = Piece{-1, 0};
   if (TMA) mbar_fence_init();
   __syncwarp();
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (kvh >= a.num_kv_heads) return;  // all KS warps of such a head slot leave together
 
-  // This CTA's run of units, [u_begin, u_end) of the page axis, and the request of its first unit:
-  // the last b with indptr[b] <= its page, 32 probes a round.
+  // This CTA's run of units, [u_begin, u_end) of the page axis, this warp's part of it, and the
+  // request of its first unit: the last b with indptr[b] <= its page, 32 probes a round.
   const int* const indptr = a.own.indptr;
   const int B = a.num_requests;
-  unsigned u_begin, u_end;
+  unsigned u_begin, u_end, w_begin, w_end;
   int axis0, b0;
   {
     int lo = 0, n = B, step = (n + 31) / 32;  // the answer is in [lo, lo + n)
@@ -308,7 +321,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
     u_begin = chunk * blockIdx.x;
     u_end = min(u_begin + chunk, units);
     if (u_begin >= u_end) return;
-    const int page = axis0 + (int)(u_begin / UPP);
+    const unsigned part = (u_end - u_begin + KS - 1) / KS;
+    w_begin = min(u_begin + part * ks, u_end);
+    w_end = min(w_begin + part, u_end);
+    const int page = axis0 + (int)(w_begin / UPP);
     while (n > 1) {
       const bool below = lane * step < n && probe <= page;
       const int last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
@@ -334,8 +350,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
   };
   load_batch();
   int key = 0, key_end = 0, first_page = 0;  // of the current request: next tile of this warp, end
-  int request = -1, slot = -1;
-  bool fresh = false, done = false;          // fresh: no tile of the request issued yet
+  int request = -1, slot = -1, cut = 0;
+  bool fresh = false, done = w_begin >= w_end;  // fresh: no tile of the request issued yet
 
   auto key_of = [&](unsigned unit) { return (int)(unit / UPP * BS + unit % UPP * kTile); };
   auto next_request = [&]() {
@@ -350,22 +366,26 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
       const int last = __shfl_sync(0xffffffffu, my_last, in_batch);
       request = batch + in_batch;
       const unsigned s0 = (unsigned)(first - axis0) * UPP, s1 = (unsigned)(end - axis0) * UPP;  // its units
-      if (request >= B || s0 >= u_end) { done = true; return; }
-      if (end <= first || s1 <= u_begin) continue;
+      if (request >= B || s0 >= w_end) { done = true; return; }
+      if (end <= first || s1 <= w_begin) continue;
       const int len = (end - first - 1) * (int)BS + last;
-      const int k0 = s0 < u_begin ? key_of(u_begin - s0) : 0;
-      key = min(k0, len) + ks * kTile;
-      key_end = s1 > u_end ? min(key_of(u_end - s0), len) : len;
+      key = s0 < w_begin ? min(key_of(w_begin - s0), len) : 0;
+      key_end = s1 > w_end ? min(key_of(w_end - s0), len) : len;
       first_page = first;
-      slot = s0 >= u_begin && s1 <= u_end ? (p.join_all ? (int)p.slot0 + 2 * p.n_ranges + request : -1)
-                                          : (int)p.slot0 + 2 * (int)blockIdx.x + (s0 < u_begin ? 0 : 1);
+      cut = 0;
+      slot = p.join_all ? (int)p.slot0 + 2 * p.n_ranges + request : -1;
+      if (s0 < w_begin || s1 > w_end) {
+        if (KS > 1) cut = (s0 < w_begin ? kHead : kTail) | (s0 < u_begin ? kBefore : 0) | (s1 > u_end ? kBehind : 0);
+        else slot = (int)p.slot0 + 2 * (int)blockIdx.x + (s0 < u_begin ? 0 : 1);
+      }
       fresh = true;
       return;
     }
   };
 
   // The next tile's description; its page numbers are on their way one tile before they are used.
-  int row_page = -1, row_entry = 0;  // lane r < 16: page and entry of row r, page -1 = none
+  int row_page = -1, row_entry = 0;  // lane r < 16: page and entry of row r as the table has it, -1 = no row
+  int row_at = -1;                   // its place in the table
   TileMeta next = {-1, 0, 0, 0};
   auto fetch = [&]() {
     next.request = -1;
@@ -374,26 +394,43 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
     next.request = request;
     next.keys = max(0, min(kTile, key_end - key));
     next.slot = slot;
-    next.flags = (fresh ? 1 : 0) | (key + KS * kTile >= key_end ? 2 : 0);
+    next.flags = (fresh ? 1 : 0) | (key + kTile >= key_end ? 2 | cut : 0);
     fresh = false;
-    row_page = -1;
+    row_at = row_page = -1;
     if (lane < next.keys) {
       const unsigned pg = (unsigned)(key + lane) / BS;
       row_entry = key + lane - (int)(pg * BS);
       const long long at = (long long)first_page + pg;
       if (at >= 0 && at < a.own.num_indices) {
+        row_at = (int)at;
         row_page = a.own.indices[at];
-        if ((unsigned)row_page >= (unsigned)a.num_blocks) {
-          if (a.checks) report(a.err, kErrBadPage, kWhereAttention, at, row_page);
-          row_page = -1;  // zeros
-        }
       }
     }
-    key += KS * kTile;
+    key += kTile;
+  };
+  // Q of a request, fetched when its first tile is issued, if the last one fetched is in use already
+  uint32_t q_next[kSteps][NT][2];
+  int q_next_at = -1;  // the tile (in order) it belongs to
+  const int r0 = (lane & 3) * 2, e0 = lane >> 2;
+  auto load_q = [&](uint32_t (*dst)[NT][2], int b) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool row = n * 8 + e0 < G;
+      const char* src = a.q + (long long)b * a.q_tok + (long long)(kvh * G + n * 8 + e0) * kRowBytes + r0 * 2;
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        dst[k][n][0] = row ? *reinterpret_cast<const uint32_t*>(src + k * 32) : 0u;
+        dst[k][n][1] = row ? *reinterpret_cast<const uint32_t*>(src + k * 32 + 16) : 0u;
+      }
+    }
   };
   auto issue = [&](int stage) {  // starts the copies of the tile described by `next`
     if (lane == 0) meta[stage] = next;
     const uint32_t base = ring + stage * S::kStage;
+    if (row_at >= 0 && (unsigned)row_page >= (unsigned)a.num_blocks) {
+      if (a.checks) report(a.err, kErrBadPage, kWhereAttention, row_at, row_page);
+      row_page = -1;  // zeros
+    }
     if (TMA) {
       if (next.request >= 0) {
         const bool any = next.keys > 0;
@@ -432,19 +469,29 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
     }
   };
 
+  int issued = 0;  // tiles
+  auto advance = [&]() {
+    issue(issued % NST);
+    if (next.request >= 0) {
+      if ((next.flags & 1) && q_next_at < 0) {
+        load_q(q_next, next.request);
+        q_next_at = issued;
+      }
+      ++issued;
+      fetch();
+    } else {
+      ++issued;
+    }
+  };
   fetch();
-#pragma unroll
-  for (int s = 0; s < NST - 1; ++s) {
-    issue(s);
-    if (next.request >= 0) fetch();
-  }
+#pragma unroll 1
+  for (int s = 0; s < NST - 1; ++s) advance();
 
   // Consumer.  A lane holds, of S^T, keys lane / 4 and lane / 4 + 8 of rows 2 (lane % 4) and the next;
   // of O^T, elements 16 m + lane / 4 and + 8 of the same rows.
   uint32_t q[kSteps][NT][2];
   float o[kSteps][NT][4], m[NT][2], l[NT][2];
   const float scale2 = a.scale * kLog2e;
-  const int r0 = (lane & 3) * 2, e0 = lane >> 2;
   // ldmatrix addresses inside a plane: row, then the lane's chunk of step 0; step k flips bits 5, 6
   const uint32_t k_addr = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
   const uint32_t v_addr = ((lane & 7) + ((lane >> 4) << 3)) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
@@ -456,24 +503,29 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
     __syncwarp();
     const TileMeta t = meta[stage];
     if (t.request < 0) break;
-    issue((it + NST - 1) % NST);
-    if (next.request >= 0) fetch();
+    advance();
     if (TMA && !dead && !mbar_wait_bounded(&full[stage], (it / NST) & 1)) {
       report(a.err, kErrWaitTimeout, kWhereAttention, blockIdx.x, it);
-      dead = true;  // goes on without waiting: the head's other warps meet it at their barrier
+      dead = true;  // goes on without waiting: the head's other warps meet it at the join's barrier
     }
 
     if (t.flags & 1) {
+      if (q_next_at == it) {
+        q_next_at = -1;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            q[k][n][0] = q_next[k][n][0];
+            q[k][n][1] = q_next[k][n][1];
+          }
+      } else {
+        load_q(q, t.request);
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const bool row = n * 8 + e0 < G;
-        const char* src = a.q + (long long)t.request * a.q_tok + (long long)(kvh * G + n * 8 + e0) * kRowBytes + r0 * 2;
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          q[k][n][0] = row ? *reinterpret_cast<const uint32_t*>(src + k * 32) : 0u;
-          q[k][n][1] = row ? *reinterpret_cast<const uint32_t*>(src + k * 32 + 16) : 0u;
-          o[k][n][0] = o[k][n][1] = o[k][n][2] = o[k][n][3] = 0.f;
-        }
+        for (int k = 0; k < kSteps; ++k) o[k][n][0] = o[k][n][1] = o[k][n][2] = o[k][n][3] = 0.f;
         m[n][0] = m[n][1] = -INFINITY;
         l[n][0] = l[n][1] = 0.f;
       }
@@ -574,7 +626,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
           l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], 8);
           l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], 16);
         }
-      if (KS == 1) {
+      if ((t.flags & (kHead | kTail)) == 0) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float inv[2];
@@ -601,9 +653,12 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
             }
         }
       } else {
-        // [warp][G][D] accumulators, then [warp][G] maxima and sums
-        float* const jm = joins + kDecodeWarps * G * D;
-        float* const jl = jm + kDecodeWarps * G;
+        // left for the join: a tail is the warp's last piece, its ring holds nothing any more
+        const int tail = t.flags & kTail ? 1 : 0;
+        float* const dst = tail ? reinterpret_cast<float*>(smem + warp * NST * S::kStage) : heads + warp * G * D;
+        float* const stat = heads + kDecodeWarps * G * D + (warp * 2 + tail) * 2 * G;
+        __syncwarp();
+        if (lane == 0) pieces[warp * 2 + tail] = Piece{t.request, t.flags};
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -611,36 +666,75 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
             const int r = n * 8 + r0 + i;
             if (r >= G) continue;
             if (e0 == 0) {
-              jm[warp * G + r] = m[n][i];
-              jl[warp * G + r] = l[n][i];
+              stat[r] = m[n][i];
+              stat[G + r] = l[n][i];
             }
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
-              joins[(warp * G + r) * D + 16 * k + e0] = o[k][n][i];
-              joins[(warp * G + r) * D + 16 * k + 8 + e0] = o[k][n][2 + i];
+              dst[r * D + 16 * k + e0] = o[k][n][i];
+              dst[r * D + 16 * k + 8 + e0] = o[k][n][2 + i];
             }
           }
-        asm volatile("bar.sync %0, %1;" ::"r"(1 + hs), "r"(KS * 32) : "memory");
-        for (int e = ks * 32 + lane; e < G * (D / 2); e += KS * 32) {
-          const int r = e / (D / 2), d = (e - r * (D / 2)) * 2;
-          float mm = -INFINITY;
-          for (int k = 0; k < KS; ++k) mm = fmaxf(mm, jm[(hs + k * HB) * G + r]);
-          float ll = 0.f, x = 0.f, y = 0.f;
-          for (int k = 0; k < KS; ++k) {
-            const int w = (hs + k * HB) * G + r;
-            const float f = jm[w] == -INFINITY ? 0.f : exp2_fast(jm[w] - mm);
-            const float2 v = *reinterpret_cast<const float2*>(joins + w * D + d);
-            ll = fmaf(f, jl[w], ll);
-            x = fmaf(f, v.x, x);
-            y = fmaf(f, v.y, y);
-          }
-          const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
-          if (t.slot >= 0) *reinterpret_cast<float2*>(po + r * D + d) = make_float2(x * inv, y * inv);
-          else *reinterpret_cast<uint32_t*>(out + r * kRowBytes + d * 2) = down2<BF16>(x * inv, y * inv);
-          if (d == 0 && lse != nullptr) lse[r] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * unit;
-        }
-        asm volatile("bar.sync %0, %1;" ::"r"(1 + hs), "r"(KS * 32) : "memory");
       }
+    }
+  }
+  if (KS > 1) {
+    // Join what the borders between this head's warps cut: pieces in order, a chain is a run of
+    // pieces of one request.  Every wait above was on a copy that is done, so the rings are free.
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + hs), "r"(KS * 32) : "memory");
+    const int head0 = kvh * G;
+    for (int first = 0; first < 2 * KS;) {
+      auto piece = [&](int i) { return pieces[(hs + (i >> 1) * HB) * 2 + (i & 1)]; };
+      const Piece start = piece(first);
+      if (start.request < 0) {
+        ++first;
+        continue;
+      }
+      int flags = 0, last = first;  // [first, last) of the chain
+      for (int i = first; i < 2 * KS; ++i) {
+        const Piece x = piece(i);
+        if (x.request >= 0 && x.request != start.request) break;
+        if (x.request >= 0) {
+          flags |= x.flags;
+          last = i + 1;
+        }
+      }
+      const int slot = flags & kBefore   ? (int)p.slot0 + 2 * (int)blockIdx.x
+                       : flags & kBehind ? (int)p.slot0 + 2 * (int)blockIdx.x + 1
+                       : p.join_all      ? (int)p.slot0 + 2 * p.n_ranges + start.request
+                                         : -1;
+      char* const out = a.out + (long long)start.request * a.o_tok + (long long)head0 * kRowBytes;
+      float* const lse = slot >= 0 ? p.part.lse + (long long)slot * a.num_heads + head0
+                         : a.lse != nullptr ? a.lse + (long long)start.request * a.num_heads + head0 : nullptr;
+      float* const po = p.part.out + ((long long)max(slot, 0) * a.num_heads + head0) * D;
+      for (int e = ks * 32 + lane; e < G * (D / 4); e += KS * 32) {
+        const int r = e / (D / 4), d = (e - r * (D / 4)) * 4;
+        float mm = -INFINITY;
+        for (int i = first; i < last; ++i)
+          if (piece(i).request >= 0) mm = fmaxf(mm, heads[kDecodeWarps * G * D + ((hs + (i >> 1) * HB) * 2 + (i & 1)) * 2 * G + r]);
+        float ll = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = first; i < last; ++i) {
+          if (piece(i).request < 0) continue;
+          const int w = hs + (i >> 1) * HB;
+          const float* stat = heads + kDecodeWarps * G * D + (w * 2 + (i & 1)) * 2 * G;
+          const float* src = i & 1 ? reinterpret_cast<const float*>(smem + w * NST * S::kStage) : heads + w * G * D;
+          const float f = stat[r] == -INFINITY ? 0.f : exp2_fast(stat[r] - mm);
+          const float4 v = *reinterpret_cast<const float4*>(src + r * D + d);
+          ll = fmaf(f, stat[G + r], ll);
+          acc.x = fmaf(f, v.x, acc.x);
+          acc.y = fmaf(f, v.y, acc.y);
+          acc.z = fmaf(f, v.z, acc.z);
+          acc.w = fmaf(f, v.w, acc.w);
+        }
+        const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+        if (slot >= 0)
+          *reinterpret_cast<float4*>(po + r * D + d) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        else
+          *reinterpret_cast<uint2*>(out + r * kRowBytes + d * 2) = make_uint2(down2<BF16>(acc.x * inv, acc.y * inv), down2<BF16>(acc.z * inv, acc.w * inv));
+        if (d == 0 && lse != nullptr) lse[r] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * (slot >= 0 ? 1.f : kLn2);
+      }
+      first = last;
     }
   }
   if (!TMA) cp_async_wait<0>();
