@@ -198,6 +198,9 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 __device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
@@ -214,9 +217,10 @@ struct Partials {
 
 // ---------------------------------------------------------------- one token a request
 // Bound by HBM: every K / V row is read once for the G = num_heads / num_kv_heads rows that share
-// it.  The pages of all requests form one axis (kv_indptr's own), cut into 16-key units; CTA x of
-// a head block takes the x-th equal run of units, whatever requests it meets, so the load is even
-// for any mix of lengths and nothing is planned on the host.  A request inside one run is
+// it.  The pages of all requests form one axis (kv_indptr's own), cut into 16-key units, with one
+// unit more a request for what its end costs; CTA x of a head block takes the x-th equal run of
+// units, whatever requests it meets, so the load is even for any mix of lengths and nothing is
+// planned on the host.  A request inside one run is
 // finished there; one cut by a border leaves a partial in each run (slot 2x if it began in an
 // earlier run, else 2x + 1) for the join kernel.
 //
@@ -298,6 +302,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
   // [warp][G][D] heads, then [warp][G] their maxima and sums; a tail takes the warp's own ring
   float* const heads = reinterpret_cast<float*>(smem + S::kRing + S::kMeta);
 
+  if (TMA && threadIdx.x < 2) prefetch_tensormap(threadIdx.x == 0 ? &p.kmap : &p.vmap);
   if (TMA && lane < NST) mbar_init(&full[lane], 1);  // the warp's own
   if (lane < 2) pieces[warp * 2 + lane] = Piece{-1, 0};
   if (TMA) mbar_fence_init();
@@ -312,11 +317,12 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
   const int B = a.num_requests;
   unsigned u_begin, u_end, w_begin, w_end;
   int axis0, b0;
+  auto place = [&](int first, int b) { return (unsigned)(first - axis0) * UPP + (unsigned)b; };  // of request b on the axis
   {
     int lo = 0, n = B, step = (n + 31) / 32;  // the answer is in [lo, lo + n)
     int probe = lane * step < n ? indptr[lane * step] : 0;
     axis0 = indptr[0];
-    const unsigned units = (unsigned)max(indptr[B] - axis0, 0) * UPP;
+    const unsigned units = place(max(indptr[B], axis0), B);
     const unsigned chunk = (units + p.n_ranges - 1) / p.n_ranges;
     u_begin = chunk * blockIdx.x;
     u_end = min(u_begin + chunk, units);
@@ -324,9 +330,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
     const unsigned part = (u_end - u_begin + KS - 1) / KS;
     w_begin = min(u_begin + part * ks, u_end);
     w_end = min(w_begin + part, u_end);
-    const int page = axis0 + (int)(w_begin / UPP);
     while (n > 1) {
-      const bool below = lane * step < n && probe <= page;
+      const bool below = lane * step < n && place(probe, lo + lane * step) <= w_begin;
       const int last = 31 - __clz(__ballot_sync(0xffffffffu, below) | 1u);
       n = min(step, n - last * step);
       lo += last * step;
@@ -365,7 +370,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
       const int end = __shfl_sync(0xffffffffu, my_end, in_batch);
       const int last = __shfl_sync(0xffffffffu, my_last, in_batch);
       request = batch + in_batch;
-      const unsigned s0 = (unsigned)(first - axis0) * UPP, s1 = (unsigned)(end - axis0) * UPP;  // its units
+      const unsigned s0 = place(first, request), s1 = s0 + (unsigned)(end - first) * UPP;  // its units
       if (request >= B || s0 >= w_end) { done = true; return; }
       if (end <= first || s1 <= w_begin) continue;
       const int len = (end - first - 1) * (int)BS + last;
@@ -683,49 +688,46 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
     // pieces of one request.  Every wait above was on a copy that is done, so the rings are free.
     asm volatile("bar.sync %0, %1;" ::"r"(1 + hs), "r"(KS * 32) : "memory");
     const int head0 = kvh * G;
-    for (int first = 0; first < 2 * KS;) {
-      auto piece = [&](int i) { return pieces[(hs + (i >> 1) * HB) * 2 + (i & 1)]; };
-      const Piece start = piece(first);
-      if (start.request < 0) {
-        ++first;
-        continue;
-      }
-      int flags = 0, last = first;  // [first, last) of the chain
-      for (int i = first; i < 2 * KS; ++i) {
-        const Piece x = piece(i);
-        if (x.request >= 0 && x.request != start.request) break;
-        if (x.request >= 0) {
-          flags |= x.flags;
-          last = i + 1;
-        }
-      }
-      const int slot = flags & kBefore   ? (int)p.slot0 + 2 * (int)blockIdx.x
-                       : flags & kBehind ? (int)p.slot0 + 2 * (int)blockIdx.x + 1
-                       : p.join_all      ? (int)p.slot0 + 2 * p.n_ranges + start.request
-                                         : -1;
-      char* const out = a.out + (long long)start.request * a.o_tok + (long long)head0 * kRowBytes;
+    // lane i < 2 KS: the i-th piece; a chain starts where a piece's request is not the last one's
+    const Piece mine = lane < 2 * KS ? pieces[(hs + (lane >> 1) * HB) * 2 + (lane & 1)] : Piece{-1, 0};
+    const unsigned valid = __ballot_sync(0xffffffffu, mine.request >= 0);
+    const unsigned before = valid & ((1u << lane) - 1u);
+    const int previous = __shfl_sync(0xffffffffu, mine.request, before != 0 ? 31 - __clz(before) : lane);
+    unsigned starts = __ballot_sync(0xffffffffu, mine.request >= 0 && (before == 0 || previous != mine.request));
+    while (starts != 0) {
+      const int first = __ffs(starts) - 1;
+      starts &= starts - 1;
+      const unsigned chain = valid & (starts != 0 ? (1u << (__ffs(starts) - 1)) - 1u : 0xffffffffu) & ~((1u << first) - 1u);
+      const bool in_chain = chain >> lane & 1;
+      const int which = __shfl_sync(0xffffffffu, mine.request, first);
+      const bool from_before = __any_sync(0xffffffffu, in_chain && (mine.flags & kBefore));
+      const bool goes_on = __any_sync(0xffffffffu, in_chain && (mine.flags & kBehind));
+      const int slot = from_before  ? (int)p.slot0 + 2 * (int)blockIdx.x
+                       : goes_on    ? (int)p.slot0 + 2 * (int)blockIdx.x + 1
+                       : p.join_all ? (int)p.slot0 + 2 * p.n_ranges + which
+                                    : -1;
+      char* const out = a.out + (long long)which * a.o_tok + (long long)head0 * kRowBytes;
       float* const lse = slot >= 0 ? p.part.lse + (long long)slot * a.num_heads + head0
-                         : a.lse != nullptr ? a.lse + (long long)start.request * a.num_heads + head0 : nullptr;
+                         : a.lse != nullptr ? a.lse + (long long)which * a.num_heads + head0 : nullptr;
       float* const po = p.part.out + ((long long)max(slot, 0) * a.num_heads + head0) * D;
       for (int e = ks * 32 + lane; e < G * (D / 4); e += KS * 32) {
         const int r = e / (D / 4), d = (e - r * (D / 4)) * 4;
-        float mm = -INFINITY;
-        for (int i = first; i < last; ++i)
-          if (piece(i).request >= 0) mm = fmaxf(mm, heads[kDecodeWarps * G * D + ((hs + (i >> 1) * HB) * 2 + (i & 1)) * 2 * G + r]);
-        float ll = 0.f;
+        float mm = -INFINITY, ll = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = first; i < last; ++i) {
-          if (piece(i).request < 0) continue;
-          const int w = hs + (i >> 1) * HB;
+        for (unsigned left = chain; left != 0; left &= left - 1) {
+          const int i = __ffs(left) - 1, w = hs + (i >> 1) * HB;
           const float* stat = heads + kDecodeWarps * G * D + (w * 2 + (i & 1)) * 2 * G;
           const float* src = i & 1 ? reinterpret_cast<const float*>(smem + w * NST * S::kStage) : heads + w * G * D;
-          const float f = stat[r] == -INFINITY ? 0.f : exp2_fast(stat[r] - mm);
           const float4 v = *reinterpret_cast<const float4*>(src + r * D + d);
-          ll = fmaf(f, stat[G + r], ll);
-          acc.x = fmaf(f, v.x, acc.x);
-          acc.y = fmaf(f, v.y, acc.y);
-          acc.z = fmaf(f, v.z, acc.z);
-          acc.w = fmaf(f, v.w, acc.w);
+          const float pm = stat[r], pl = stat[G + r];
+          if (pm == -INFINITY) continue;  // a piece without a key
+          const float top = fmaxf(mm, pm), keep = exp2_fast(mm - top), f = exp2_fast(pm - top);
+          mm = top;
+          ll = fmaf(ll, keep, f * pl);
+          acc.x = fmaf(acc.x, keep, f * v.x);
+          acc.y = fmaf(acc.y, keep, f * v.y);
+          acc.z = fmaf(acc.z, keep, f * v.z);
+          acc.w = fmaf(acc.w, keep, f * v.w);
         }
         const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
         if (slot >= 0)
@@ -734,7 +736,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
           *reinterpret_cast<uint2*>(out + r * kRowBytes + d * 2) = make_uint2(down2<BF16>(acc.x * inv, acc.y * inv), down2<BF16>(acc.z * inv, acc.w * inv));
         if (d == 0 && lse != nullptr) lse[r] = ll == 0.f ? -INFINITY : (mm + log2f(ll)) * (slot >= 0 ? 1.f : kLn2);
       }
-      first = last;
+      __syncwarp();
     }
   }
   if (!TMA) cp_async_wait<0>();
@@ -1023,6 +1025,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     mbar_init(&bars.done, 1);
     mbar_fence_init();
   }
+  if (p.box > 0 && warp == 9 && lane < 2) prefetch_tensormap(lane == 0 ? &p.kmap : &p.vmap);
   if (warp == 10) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&bars.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -1481,11 +1484,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const J
   if (p.runs) {
     const int* indptr = a.own.indptr;
     const int axis0 = indptr[0], begin = indptr[t], end = indptr[t + 1];
-    const unsigned units = (unsigned)max(indptr[a.num_requests] - axis0, 0) * p.units_per_page;
+    const unsigned units = (unsigned)max(indptr[a.num_requests] - axis0, 0) * p.units_per_page + a.num_requests;
     const unsigned chunk = (units + p.n_ranges - 1) / p.n_ranges;
-    if (end > begin && chunk > 0) {  // the runs that hold a part of the request
-      x0 = (int)min((unsigned)(begin - axis0) * p.units_per_page / chunk, p.n_ranges - 1u);
-      n_runs = (int)min(((unsigned)(end - axis0) * p.units_per_page - 1) / chunk, p.n_ranges - 1u) - x0 + 1;
+    if (end > begin) {  // the runs that hold a part of the request
+      const unsigned s0 = (unsigned)(begin - axis0) * p.units_per_page + t;
+      x0 = (int)min(s0 / chunk, p.n_ranges - 1u);
+      n_runs = (int)min((s0 + (unsigned)(end - begin) * p.units_per_page - 1) / chunk, p.n_ranges - 1u) - x0 + 1;
       if (n_runs == 1 && !p.all) return;  // finished by its run
     }
   }
