@@ -244,8 +244,22 @@ struct DecodeParams {
   int units_per_page;  // 16-key units of a page
   int box;             // keys of a TMA box
   long long slot0;     // first slot of the runs
-  bool join_all;       // whole requests too go to a slot (behind the runs' own): a prefix follows
+  bool join_all;       // whole requests too go to a slot (behind the runs' own): the prefix is joined
+  bool beside;         // runs beside the kernel before it, see wait_before
 };
+
+// Programmatic launches.  A kernel normally waits for the one before it (and lets the one behind it
+// get ready).  The kernel of the own keys needs nothing that the kernel of the shared prefix in
+// front of it writes, only what that one has itself waited for before it let this one start: it
+// runs beside it, on the SMs that are free, and waits behind its work instead, so that what follows
+// (the join) still finds both done.
+__device__ __forceinline__ void wait_before(bool beside) {
+  if (!beside) asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_behind(bool beside) {
+  if (beside) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 struct __align__(16) TileMeta {
   int request;  // -1: behind the last tile
@@ -307,9 +321,11 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
   if (lane < 2) pieces[warp * 2 + lane] = Piece{-1, 0};
   if (TMA) mbar_fence_init();
   __syncwarp();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (kvh >= a.num_kv_heads) return;  // all KS warps of such a head slot leave together
+  wait_before(p.beside);
+  if (kvh >= a.num_kv_heads) {  // all KS warps of such a head slot leave together
+    wait_behind(p.beside);
+    return;
+  }
 
   // This CTA's run of units, [u_begin, u_end) of the page axis, this warp's part of it, and the
   // request of its first unit: the last b with indptr[b] <= its page, 32 probes a round.
@@ -326,7 +342,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
     const unsigned chunk = (units + p.n_ranges - 1) / p.n_ranges;
     u_begin = chunk * blockIdx.x;
     u_end = min(u_begin + chunk, units);
-    if (u_begin >= u_end) return;
+    if (u_begin >= u_end) {
+      wait_behind(p.beside);
+      return;
+    }
     const unsigned part = (u_end - u_begin + KS - 1) / KS;
     w_begin = min(u_begin + part * ks, u_end);
     w_end = min(w_begin + part, u_end);
@@ -744,6 +763,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
   // is in flight when the CTA leaves.
   if (TMA && dead)
     for (int i = max(0, it - NST); i < it; ++i) mbar_wait_bounded(&full[i % NST], (i / NST) & 1);
+  wait_behind(p.beside);
 }
 
 // ---------------------------------------------------------------- tiles of rows
@@ -785,6 +805,7 @@ struct TileParams {
   int slot0;          // first of n_splits sets of partials ([num_tokens] slots each), -1: final
   int causal;
   int box;            // keys of a TMA box, 0 = no TMA
+  bool beside;        // see wait_before
 };
 
 template <int D>
@@ -1034,8 +1055,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  wait_before(p.beside);
 
   const uint32_t sm_q = smem + S::kQ, sm_k = smem + S::kK, sm_v = smem + S::kV;
   // The sign of the scale goes into Q; a scale of 0 must still leave masked scores at -infinity.
@@ -1445,6 +1465,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
   __syncthreads();
   tc_fence_after();
   if (warp == 10) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  wait_behind(p.beside);
 }
 
 // ---------------------------------------------------------------- join
@@ -1675,7 +1696,7 @@ cudaError_t launch_decode(const AttentionParams& p, const Plan& plan, bool pdl, 
   d.hb_shift = plan.hb_shift;
   d.units_per_page = plan.units_per_page;
   d.slot0 = (long long)(plan.shared_splits + plan.own_splits) * p.num_tokens;
-  d.join_all = plan.shared_splits > 0;
+  d.join_all = d.beside = plan.shared_splits > 0;
   const int G = p.num_heads / p.num_kv_heads, HB = 1 << plan.hb_shift;
   d.box = p.block_size % kTile == 0 ? kTile : p.block_size == 8 ? 8 : 0;
   const bool tma = d.box > 0 && encode_plane(p, p.kcache, d.box, &d.kmap) && encode_plane(p, p.vcache, d.box, &d.vmap);
@@ -1703,6 +1724,7 @@ cudaError_t launch_tile(const AttentionParams& p, const Plan& plan, bool shared,
   t.n_slots = (int)slots;
   t.slot0 = plan.join ? (shared ? 0 : plan.shared_splits) : -1;
   t.causal = !shared && p.causal;
+  t.beside = !shared && plan.shared_splits > 0;
   const int bs = p.block_size;
   if (bs % kKeys == 0) t.box = kKeys;
   else if (bs >= 8 && bs < kKeys && kKeys % bs == 0) t.box = bs;
