@@ -1483,25 +1483,23 @@ struct JoinParams {
 };
 constexpr int kJoinWarps = 8;
 
-template <bool BF16, int D>
+// HPW rows (heads of one token) a warp: one where there are few rows, so that their parts are the
+// parallel loads, four where there are many.
+template <bool BF16, int D, int HPW>
 __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const JoinParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const AttentionParams& a = p.a;
   const int lane = threadIdx.x & 31;
-  const int t = blockIdx.x, h = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
-  if (h >= a.num_heads) return;
-  int first = 0;  // parts of the row: sets [first, n_sets), then n_runs slots of the runs
-  if (a.qo_indptr != nullptr && (t < a.qo_indptr[0] || t >= a.qo_indptr[a.num_requests])) return;  // left as it is
-  if (p.n_shared > 0 && a.group_indptr != nullptr) {
-    // a request outside every group has no set from the prefix
-    const int b0 = min(max(a.group_indptr[0], 0), a.num_requests);
-    const int b1 = min(max(a.group_indptr[a.num_groups], 0), a.num_requests);
-    const int t0 = a.qo_indptr != nullptr ? a.qo_indptr[b0] : b0, t1 = a.qo_indptr != nullptr ? a.qo_indptr[b1] : b1;
-    if (t < t0 || t >= t1) first = p.n_shared;
-  }
-  const long long slot0 = (long long)p.n_sets * a.num_tokens;
-  int n_runs = 0, x0 = 0;
+  const int t = blockIdx.x, h0 = (blockIdx.y * kJoinWarps + (threadIdx.x >> 5)) * HPW;
+  if (h0 >= a.num_heads) return;
+  int first = 0;  // parts of a row: sets [first, n_sets), then n_runs slots of the runs
+  int x0 = 0, n_runs = 0;
+  const bool grouped = p.n_shared > 0 && a.group_indptr != nullptr;
+  const int q_first = a.qo_indptr != nullptr ? a.qo_indptr[0] : 0;
+  const int q_last = a.qo_indptr != nullptr ? a.qo_indptr[a.num_requests] : a.num_tokens;
+  const int b0 = grouped ? min(max(a.group_indptr[0], 0), a.num_requests) : 0;
+  const int b1 = grouped ? min(max(a.group_indptr[a.num_groups], 0), a.num_requests) : 0;
   if (p.runs) {
     const int* indptr = a.own.indptr;
     const int axis0 = indptr[0], begin = indptr[t], end = indptr[t + 1];
@@ -1510,63 +1508,93 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const J
     if (end > begin) {  // the runs that hold a part of the request
       const unsigned s0 = (unsigned)(begin - axis0) * p.units_per_page + t;
       x0 = (int)min(s0 / chunk, p.n_ranges - 1u);
-      n_runs = (int)min((s0 + (unsigned)(end - begin) * p.units_per_page - 1) / chunk, p.n_ranges - 1u) - x0 + 1;
+      n_runs = max((int)min((s0 + (unsigned)(end - begin) * p.units_per_page - 1) / chunk, p.n_ranges - 1u) - x0 + 1, 0);
       if (n_runs == 1 && !p.all) return;  // finished by its run
     }
   }
-  const int n_set = p.n_sets - first, n = n_set + max(n_runs, 0);
+  if (t < q_first || t >= q_last) return;  // left as it is
+  if (grouped) {
+    // a request outside every group has no set from the prefix
+    const int t0 = a.qo_indptr != nullptr ? a.qo_indptr[b0] : b0, t1 = a.qo_indptr != nullptr ? a.qo_indptr[b1] : b1;
+    if (t < t0 || t >= t1) first = p.n_shared;
+  }
+  const long long slot0 = (long long)p.n_sets * a.num_tokens;
+  const int n_set = p.n_sets - first, n = n_set + n_runs;
   auto slot_of = [&](int i) -> long long {
     if (i < n_set) return (long long)(first + i) * a.num_tokens + t;
     if (n_runs == 1) return slot0 + 2 * p.n_ranges + t;  // whole
     const int x = i - n_set;
     return slot0 + 2 * (x0 + x) + (x == 0 ? 1 : 0);
   };
-  constexpr int E = D / 32;
-  float acc[E] = {}, m = -INFINITY, l = 0.f;
-  for (int base = 0; base < n; base += 32) {
+  constexpr int E = D / 32, kLook = 32 / HPW, kBatch = 8 / HPW;  // parts looked up / loaded at once
+  float acc[HPW][E] = {}, m = -INFINITY, l = 0.f;  // m, l: of the head this lane looks up
+  const int hh = lane / kLook;
+  for (int base = 0; base < n; base += kLook) {
+    const int count = min(kLook, n - base);
     long long at = 0;
     float s = -INFINITY;
-    if (base + lane < n) {
-      at = slot_of(base + lane) * a.num_heads + h;
-      s = p.part.lse[at];
+    if (lane % kLook < count) {
+      at = slot_of(base + lane % kLook) * a.num_heads;
+      if (h0 + hh < a.num_heads) s = p.part.lse[at + h0 + hh];
     }
     float top = fmaxf(s, m);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float w = s == -INFINITY ? 0.f : exp2_fast(s - top);  // a part without a key was not written
-    if (m != -INFINITY) {
-      const float keep = exp2_fast(m - top);
-      l *= keep;
+    for (int o = kLook / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // NaN counts as a part (its row is NaN); a part without a key was not written
+    const float w = s == -INFINITY ? 0.f : exp2_fast(s - top);
+    const float keep = m == -INFINITY ? 0.f : exp2_fast(m - top);
+    float sum = w;
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] *= keep;
-    }
+    for (int o = kLook / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    l = fmaf(l, keep, sum);
     m = top;
-    const unsigned live = __ballot_sync(0xffffffffu, w != 0.f);
-#pragma unroll 4
-    for (int i = 0; i < min(32, n - base); ++i) {
-      const float wi = __shfl_sync(0xffffffffu, w, i);
-      const long long ai = __shfl_sync(0xffffffffu, at, i);
-      l += wi;
-      float v[E] = {};
-      if (live >> i & 1) {
-        if constexpr (E == 4) {
-          const float4 x = *reinterpret_cast<const float4*>(p.part.out + ai * D + lane * E);
-          v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-        } else {
-          const float2 x = *reinterpret_cast<const float2*>(p.part.out + ai * D + lane * E);
-          v[0] = x.x; v[1] = x.y;
+#pragma unroll
+    for (int x = 0; x < HPW; ++x) {
+      const float k = __shfl_sync(0xffffffffu, keep, x * kLook);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[x][e] *= k;
+    }
+    for (int i = 0; i < count; i += kBatch) {
+      float v[kBatch][HPW][E];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const long long slot = __shfl_sync(0xffffffffu, at, min(i + u, count - 1));
+#pragma unroll
+        for (int x = 0; x < HPW; ++x) {
+          const float* src = p.part.out + (slot + min(h0 + x, a.num_heads - 1)) * D + lane * E;
+          if constexpr (E == 4) {
+            const float4 f = *reinterpret_cast<const float4*>(src);
+            v[u][x][0] = f.x; v[u][x][1] = f.y; v[u][x][2] = f.z; v[u][x][3] = f.w;
+          } else {
+            const float2 f = *reinterpret_cast<const float2*>(src);
+            v[u][x][0] = f.x; v[u][x][1] = f.y;
+          }
         }
       }
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(wi, v[e], acc[e]);
+      for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+        for (int x = 0; x < HPW; ++x) {
+          const float wi = i + u < count ? __shfl_sync(0xffffffffu, w, x * kLook + min(i + u, count - 1)) : 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[x][e] = fmaf(wi, wi == 0.f ? 0.f : v[u][x][e], acc[x][e]);
+        }
     }
   }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  uint32_t* out = reinterpret_cast<uint32_t*>(a.out + (long long)t * a.o_tok + ((long long)h * D + lane * E) * 2);
 #pragma unroll
-  for (int e = 0; e < E; e += 2) out[e / 2] = down2<BF16>(acc[e] * inv, acc[e + 1] * inv);
-  if (a.lse != nullptr && lane == 0)
-    a.lse[(long long)t * a.num_heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  for (int x = 0; x < HPW; ++x) {
+    const float total = __shfl_sync(0xffffffffu, l, x * kLook), most = __shfl_sync(0xffffffffu, m, x * kLook);
+    if (h0 + x >= a.num_heads) continue;
+    const float inv = total > 0.f ? 1.f / total : (total == 0.f ? 0.f : total);
+    uint32_t* out = reinterpret_cast<uint32_t*>(a.out + (long long)t * a.o_tok + ((long long)(h0 + x) * D + lane * E) * 2);
+    uint32_t r[E / 2];
+#pragma unroll
+    for (int e = 0; e < E; e += 2) r[e / 2] = down2<BF16>(acc[x][e] * inv, acc[x][e + 1] * inv);
+    if constexpr (E == 4) *reinterpret_cast<uint2*>(out) = make_uint2(r[0], r[1]);
+    else out[0] = r[0];
+    if (a.lse != nullptr && lane == 0)
+      a.lse[(long long)t * a.num_heads + h0 + x] = total == 0.f ? -INFINITY : (most + log2f(total)) * kLn2;
+  }
 }
 
 // ---------------------------------------------------------------- launch rules
@@ -1741,7 +1769,7 @@ cudaError_t launch_tile(const AttentionParams& p, const Plan& plan, bool shared,
 }
 
 template <bool BF16, int D>
-cudaError_t launch_join(const AttentionParams& p, const Plan& plan, bool pdl, cudaStream_t stream) {
+cudaError_t launch_join(const AttentionParams& p, const Plan& plan, int sms, bool pdl, cudaStream_t stream) {
   JoinParams j{};
   j.a = p;
   j.part = partials_at(p, plan);
@@ -1751,8 +1779,11 @@ cudaError_t launch_join(const AttentionParams& p, const Plan& plan, bool pdl, cu
   j.all = plan.shared_splits > 0;
   j.n_ranges = plan.n_ranges;
   j.units_per_page = plan.units_per_page;
-  Launch go(dim3(p.num_tokens, (p.num_heads + kJoinWarps - 1) / kJoinWarps), kJoinWarps * 32, 0, pdl, stream);
-  return cudaLaunchKernelEx(&go.cfg, attention_join_kernel<BF16, D>, j);
+  // four rows a warp once one a warp would not fit the GPU at once (64 warps an SM)
+  const bool many = (long long)p.num_tokens * p.num_heads > 64ll * sms;
+  const int heads = kJoinWarps * (many ? 4 : 1);
+  Launch go(dim3(p.num_tokens, (p.num_heads + heads - 1) / heads), kJoinWarps * 32, 0, pdl, stream);
+  return cudaLaunchKernelEx(&go.cfg, many ? attention_join_kernel<BF16, D, 4> : attention_join_kernel<BF16, D, 1>, j);
 }
 
 template <bool BF16>
@@ -1764,7 +1795,7 @@ cudaError_t launch_rows(const AttentionParams& p, bool pdl, cudaStream_t stream)
 }
 
 template <bool BF16, int D>
-cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, bool pdl, int* launches, cudaStream_t stream) {
+cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, int sms, bool pdl, int* launches, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
   if (plan.shared_splits > 0) {
     e = launch_tile<BF16, D>(p, plan, true, pdl, stream);
@@ -1780,20 +1811,20 @@ cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, bool pdl, 
     *launches += e == cudaSuccess;
   }
   if (e == cudaSuccess && plan.join) {
-    e = launch_join<BF16, D>(p, plan, pdl, stream);
+    e = launch_join<BF16, D>(p, plan, sms, pdl, stream);
     *launches += e == cudaSuccess;
   }
   return e;
 }
 
 template <bool BF16>
-cudaError_t launch_typed(const AttentionParams& p, const Plan& plan, bool pdl, int* launches, cudaStream_t stream) {
+cudaError_t launch_typed(const AttentionParams& p, const Plan& plan, int sms, bool pdl, int* launches, cudaStream_t stream) {
   if (plan.rows) {
     *launches = 1;
     return launch_rows<BF16>(p, pdl, stream);
   }
-  return p.head_dim == 64 ? launch_matrix<BF16, 64>(p, plan, pdl, launches, stream)
-                          : launch_matrix<BF16, 128>(p, plan, pdl, launches, stream);
+  return p.head_dim == 64 ? launch_matrix<BF16, 64>(p, plan, sms, pdl, launches, stream)
+                          : launch_matrix<BF16, 128>(p, plan, sms, pdl, launches, stream);
 }
 
 }  // namespace
@@ -1807,8 +1838,8 @@ long long attention_workspace_bytes(const AttentionParams& p, int sms) {
 cudaError_t launch_attention(const AttentionParams& p, int sms, bool pdl, int* launches, cudaStream_t stream) {
   const Plan plan = plan_of(p, sms);
   *launches = 0;
-  return p.is_bf16 ? launch_typed<true>(p, plan, pdl, launches, stream)
-                   : launch_typed<false>(p, plan, pdl, launches, stream);
+  return p.is_bf16 ? launch_typed<true>(p, plan, sms, pdl, launches, stream)
+                   : launch_typed<false>(p, plan, sms, pdl, launches, stream);
 }
 
 }  // namespace lms
