@@ -793,7 +793,6 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
 constexpr int kRows = 128;       // rows of a tile
 constexpr int kKeys = 128;       // keys of a tile
 constexpr int kTileThreads = 384;
-__device__ constexpr bool kEmulated[8] = {false, false, true, false, false, false, true, false};
 
 struct TileParams {
   CUtensorMap kmap, vmap;
@@ -876,27 +875,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {  // NaN if on
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-// 2^x of two values on the FMA pipe, for 2^-126 <= 2^x < 2^127 (smaller ones give 2^-126): n = x
-// rounded to the nearest integer by adding 1.5 * 2^23, whose sum carries n in its low bits, then 2^(x - n)
-// by the polynomial of degree 5 with the smallest relative error on [-1/2, 1/2] (2.1e-7 evaluated in
-// fp32, that of the special-function unit), then n into the exponent.
-__device__ __forceinline__ float2 exp2_poly(uint64_t x) {
-  float2 v = unpack2(x);
-  const uint64_t a = pack2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
-  const uint64_t t = add2(a, pack2(12582912.f, 12582912.f));
-  const uint64_t n = add2(t, pack2(-12582912.f, -12582912.f));
-  const uint64_t f = fma2(n, pack2(-1.f, -1.f), a);
-  uint64_t p = pack2(0.001327647129073739f, 0.001327647129073739f);
-  p = fma2(p, f, pack2(0.009675541892647743f, 0.009675541892647743f));
-  p = fma2(p, f, pack2(0.05550713092088699f, 0.05550713092088699f));
-  p = fma2(p, f, pack2(0.24022120237350464f, 0.24022120237350464f));
-  p = fma2(p, f, pack2(0.6931469440460205f, 0.6931469440460205f));
-  p = fma2(p, f, pack2(1.0000001192092896f, 1.0000001192092896f));
-  v = unpack2(p);
-  const float2 e = unpack2(t);
-  return make_float2(__uint_as_float(__float_as_uint(v.x) + (__float_as_uint(e.x) << 23)),
-                     __uint_as_float(__float_as_uint(v.y) + (__float_as_uint(e.y) << 23)));
 }
 __device__ __forceinline__ void tc_ld16(uint32_t* r, uint32_t addr) {
   asm volatile(
@@ -1140,8 +1118,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           for (int c = 0; c < kKeys; c += 32) tc_ld32(raw + c, t_s + c);
           tc_wait_ld();
           const int seen = limit - (k.tile0 + j) * kKeys;
-          const bool whole = __all_sync(0xffffffffu, seen >= kKeys);  // no key of the tile is masked
-          if (!whole) {
+          if (!__all_sync(0xffffffffu, seen >= kKeys)) {
 #pragma unroll
             for (int c = 0; c < kKeys; ++c)
               if (c >= seen) s[c] = -INFINITY;
@@ -1175,36 +1152,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           const uint64_t scale_2 = pack2(scale2, scale2), base_2 = pack2(-base, -base);
           uint64_t sums[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
           // P goes out in two halves, so that the products of the first run beside the second's
-          // exponentials.  Where no key is masked, 2 of every 8 pairs take the FMA pipe: the
-          // special-function unit alone (16 values a clock) would need as long as the four products.
-          auto weights = [&](auto poly) {
+          // exponentials.  (Every exponential takes the special-function unit: moving a quarter of
+          // them to a polynomial on the FMA pipe changed nothing, 236 to 247 us either way.)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              uint32_t w[kKeys / 4];
+          for (int half = 0; half < 2; ++half) {
+            uint32_t w[kKeys / 4];
 #pragma unroll
-              for (int c = 0; c < kKeys / 4; ++c) {
-                const int at = half * (kKeys / 2) + 2 * c;
-                const uint64_t x = fma2(pack2(s[at], s[at + 1]), scale_2, base_2);
-                float2 e;
-                if (decltype(poly)::value && kEmulated[c % 8]) {
-                  e = exp2_poly(x);
-                } else {
-                  e = unpack2(x);
-                  e.x = exp2_fast(e.x);
-                  e.y = exp2_fast(e.y);
-                }
-                sums[c & 1] = add2(sums[c & 1], pack2(e.x, e.y));
-                w[c] = down2<BF16>(e.x, e.y);
-              }
-              tc_st32(t_s + half * 32, w);
-              tc_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&bars.pfull[i][half]);
+            for (int c = 0; c < kKeys / 4; ++c) {
+              const int at = half * (kKeys / 2) + 2 * c;
+              const float2 x = unpack2(fma2(pack2(s[at], s[at + 1]), scale_2, base_2));
+              const float x0 = exp2_fast(x.x), x1 = exp2_fast(x.y);
+              sums[c & 1] = add2(sums[c & 1], pack2(x0, x1));
+              w[c] = down2<BF16>(x0, x1);
             }
-          };
-          if (whole) weights(std::true_type{});
-          else weights(std::false_type{});
+            tc_st32(t_s + half * 32, w);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.pfull[i][half]);
+          }
           const float2 sum = unpack2(add2(sums[0], sums[1]));
           l = fmaf(l, keep, sum.x + sum.y);
         } else if (lane == 0) {
