@@ -1123,6 +1123,32 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             for (int c = 0; c < kKeys; ++c)
               if (c >= seen) s[c] = -INFINITY;
           }
+          // P goes out in two parts, so that the products of the first (3/4) run beside the second's
+          // exponentials.  The first 64 keys' exponentials start from the maximum as it was, beside
+          // the search for the tile's own; only where that is too far above (the first tile, and few
+          // others) are they done again from the new one, after O has been rescaled.
+          uint32_t w[kKeys / 2];
+          uint64_t sums[2];
+          const uint64_t scale_2 = pack2(scale2, scale2);
+          auto weights = [&](int from, int to) {  // of the pairs [from, to)
+            const float base = m == -INFINITY ? 0.f : m;
+            const uint64_t base_2 = pack2(-base, -base);
+#pragma unroll
+            for (int c = 0; c < kKeys / 2; ++c) {
+              if (c < from || c >= to) continue;
+              const float2 x = unpack2(fma2(pack2(s[2 * c], s[2 * c + 1]), scale_2, base_2));
+              const float x0 = exp2_fast(x.x), x1 = exp2_fast(x.y);
+              sums[c & 1] = c < 2 ? pack2(x0, x1) : add2(sums[c & 1], pack2(x0, x1));
+              w[c] = down2<BF16>(x0, x1);
+            }
+          };
+          auto publish = [&](int part) {
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.pfull[i][part]);
+          };
+          weights(0, 32);
           float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
           for (int c = 4; c + 8 <= kKeys; c += 8)
@@ -1132,47 +1158,35 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           for (int e = 0; e < 4; ++e) tops[e] = max3(tops[e], s[kKeys - 4 + e], tops[0]);
           float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
           top = top == -INFINITY ? top : top * scale2;
-          float keep = 1.f;
-          if (!(top <= m + kLazy)) {  // a NaN score, too, moves it: the row is NaN from here on
-            keep = exp2_fast(m - top);
-            m = top;
-          }
-          if (__any_sync(0xffffffffu, keep != 1.f) && j > 0) {
+          if (__any_sync(0xffffffffu, !(top <= m + kLazy))) {
+            float keep = 1.f;
+            if (!(top <= m + kLazy)) {  // a NaN score, too, moves it: the row is NaN from here on
+              keep = exp2_fast(m - top);
+              m = top;
+            }
+            l *= keep;
+            if (j > 0) {
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
-              uint32_t o[16];
-              tc_ld16(o, t_o + c);
-              tc_wait_ld();
+              for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                tc_ld16(o, t_o + c);
+                tc_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-              tc_st16(t_o + c, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                tc_st16(t_o + c, o);
+              }
             }
+            weights(0, 32);
           }
-          const float base = m == -INFINITY ? 0.f : m;
-          const uint64_t scale_2 = pack2(scale2, scale2), base_2 = pack2(-base, -base);
-          uint64_t sums[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
-          // P goes out in two halves, so that the products of the first run beside the second's
-          // exponentials.  (Every exponential takes the special-function unit: moving a quarter of
-          // them to a polynomial on the FMA pipe changed nothing, 236 to 247 us either way.)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t w[kKeys / 4];
-#pragma unroll
-            for (int c = 0; c < kKeys / 4; ++c) {
-              const int at = half * (kKeys / 2) + 2 * c;
-              const float2 x = unpack2(fma2(pack2(s[at], s[at + 1]), scale_2, base_2));
-              const float x0 = exp2_fast(x.x), x1 = exp2_fast(x.y);
-              sums[c & 1] = add2(sums[c & 1], pack2(x0, x1));
-              w[c] = down2<BF16>(x0, x1);
-            }
-            tc_st32(t_s + half * 32, w);
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.pfull[i][half]);
-          }
+          tc_st32(t_s, w);
+          weights(32, 48);
+          tc_st16(t_s + 32, w + 32);
+          publish(0);
+          weights(48, 64);
+          tc_st16(t_s + 48, w + 48);
+          publish(1);
           const float2 sum = unpack2(add2(sums[0], sums[1]));
-          l = fmaf(l, keep, sum.x + sum.y);
+          l += sum.x + sum.y;
         } else if (lane == 0) {
           mbar_arrive(&bars.pfull[i][0]);
           mbar_arrive(&bars.pfull[i][1]);
@@ -1339,7 +1353,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             if (ok && one) {
               const uint32_t b_low = v_low + s * (S::kStage >> 4);
 #pragma unroll
-              for (int c = half * (kKeys / 32); c < (half + 1) * (kKeys / 32); ++c)
+              for (int c = half * (kKeys / 64 * 3); c < (half ? kKeys / 16 : kKeys / 64 * 3); ++c)
                 umma_ts<id_o>(tmem + 256 + i * 128, tmem + i * 128 + c * 8, b_low + c * (2048 >> 4), c > 0 ? 1u : (uint32_t)j);
             }
             __syncwarp();
