@@ -1087,20 +1087,27 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         continue;
       }
       if (i * kRows >= k.rows) continue;  // one row tile only
-      {  // the row of Q; rows that do not exist are zeros
-        const char* src = a.q + (long long)(k.t_begin + tok) * a.q_tok + (long long)(k.kvh * G + g) * D * 2;
-        uint4 qv[D / 8];
+      {
+        // The warp's 32 rows of Q, whole lines an instruction, all of them on their way before the
+        // first is stored; rows that do not exist are zeros.
+        constexpr int kChunks = D / 8, kAtOnce = 32 / kChunks;
+        const char* const mine = a.q + (long long)(k.t_begin + tok) * a.q_tok + (long long)(k.kvh * G + g) * D * 2;
+        const int c = lane % kChunks;
+        uint4 qv[32 / kAtOnce];
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          qv[c] = make_uint4(0, 0, 0, 0);
-          if (has_row) qv[c] = *reinterpret_cast<const uint4*>(src + c * 16);
+        for (int x = 0; x < 32 / kAtOnce; ++x) {
+          const int row = x * kAtOnce + lane / kChunks;
+          const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), row));
+          qv[x] = make_uint4(0, 0, 0, 0);
+          if ((r & ~31) + row < k.rows) qv[x] = *reinterpret_cast<const uint4*>(src + c * 16);
         }
-        const int row = r & (kRows - 1);
-        const uint32_t dst = sm_q + i * kRows * D * 2 + row * 128;
+        const uint32_t dst = sm_q + i * kRows * D * 2 + (c >> 3) * (kRows * 128) + (warp & 3) * 32 * 128;
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * (kRows * 128) + (((c & 7) ^ (row & 7)) << 4)),
-                       "r"(qv[c].x ^ flip), "r"(qv[c].y ^ flip), "r"(qv[c].z ^ flip), "r"(qv[c].w ^ flip) : "memory");
+        for (int x = 0; x < 32 / kAtOnce; ++x) {
+          const int row = x * kAtOnce + lane / kChunks;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + row * 128 + (((c & 7) ^ (row & 7)) << 4)),
+                       "r"(qv[x].x ^ flip), "r"(qv[x].y ^ flip), "r"(qv[x].z ^ flip), "r"(qv[x].w ^ flip) : "memory");
+        }
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.qfull[i]);
@@ -1211,38 +1218,45 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                                   : a.out + (long long)(k.t_begin + tok) * a.o_tok + (long long)(k.kvh * G + g) * D * 2;
 #pragma unroll 1
           for (int pass = 0; pass < D / kCols; ++pass) {
+            uint32_t o[kCols];
 #pragma unroll
-            for (int c = 0; c < kCols; c += 32) {
-              uint32_t o[32];
-              tc_ld32(o, t_o + pass * kCols + c);
-              tc_wait_ld();
+            for (int c = 0; c < kCols; c += 32) tc_ld32(o + c, t_o + pass * kCols + c);
+            tc_wait_ld();
+            float odd[4] = {0.f, 0.f, 0.f, 0.f};  // NaN where an element is not finite
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                finite = fmaf(__uint_as_float(o[e]), 0.f, finite);
-                o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
-              }
-              constexpr int kPer = PART ? 4 : 8;  // values of a 16-byte chunk
+            for (int c = 0; c < kCols; ++c) {
+              odd[c & 3] = fmaf(__uint_as_float(o[c]), 0.f, odd[c & 3]);
+              o[c] = __float_as_uint(__uint_as_float(o[c]) * inv);
+            }
+            finite += (odd[0] + odd[1]) + (odd[2] + odd[3]);
+            constexpr int kPer = PART ? 4 : 8;  // values of a 16-byte chunk
 #pragma unroll
-              for (int e = 0; e < 32; e += kPer) {
-                uint32_t v[4];
+            for (int e = 0; e < kCols; e += kPer) {
+              uint32_t v[4];
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
-                  v[x] = PART ? o[e + x] : down2<BF16>(__uint_as_float(o[(e + 2 * x) & 31]), __uint_as_float(o[(e + 2 * x + 1) & 31]));
-                const int chunk = (c + e) / kPer;
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + (chunk >> 3) * (kRows * 128) + lane * 128 + (((chunk & 7) ^ (lane & 7)) << 4)),
-                             "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-              }
+              for (int x = 0; x < 4; ++x)
+                v[x] = PART ? o[e + x] : down2<BF16>(__uint_as_float(o[(e + 2 * x) % kCols]), __uint_as_float(o[(e + 2 * x + 1) % kCols]));
+              const int chunk = e / kPer;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + (chunk >> 3) * (kRows * 128) + lane * 128 + (((chunk & 7) ^ (lane & 7)) << 4)),
+                           "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
             }
             __syncwarp();
-#pragma unroll 4
-            for (int at = 0; at < 32; at += kAtOnce) {
-              const int row = at + lane / kChunks, chunk = lane % kChunks;
-              uint32_t v[4];
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                           : "r"(stage + (chunk >> 3) * (kRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) : "memory");
-              char* const dst = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), row));
-              if (have >> row & 1)
-                *reinterpret_cast<uint4*>(dst + pass * kPassBytes + chunk * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+            const int chunk = lane % kChunks;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              uint4 v[16 / kAtOnce];
+#pragma unroll
+              for (int x = 0; x < 16 / kAtOnce; ++x) {
+                const int row = half * 16 + x * kAtOnce + lane / kChunks;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[x].x), "=r"(v[x].y), "=r"(v[x].z), "=r"(v[x].w)
+                             : "r"(stage + (chunk >> 3) * (kRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) : "memory");
+              }
+#pragma unroll
+              for (int x = 0; x < 16 / kAtOnce; ++x) {
+                const int row = half * 16 + x * kAtOnce + lane / kChunks;
+                char* const dst = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), row));
+                if (have >> row & 1) *reinterpret_cast<uint4*>(dst + pass * kPassBytes + chunk * 16) = v[x];
+              }
             }
             __syncwarp();
           }
