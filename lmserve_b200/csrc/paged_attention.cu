@@ -1449,6 +1449,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       const long long kv_tiles = (k_end + kKeys - 1) / kKeys;
       k.tile0 = (int)(kv_tiles * k.split / p.n_splits);
       k.n_kv = (int)(kv_tiles * (k.split + 1) / p.n_splits) - k.tile0;
+      if (k.n_kv > 0)  // its rows of Q, on their way into L2 before the softmax warps ask for them
+        for (int x = lane; x < k.rows; x += 32) {
+          const int tok = (k.row0 + x) / G, g = k.row0 + x - tok * G;
+          const char* src = a.q + (long long)(k.t_begin + tok) * a.q_tok + (long long)(k.kvh * G + g) * D * 2;
+          prefetch_l2(src);
+          if (D > 64) prefetch_l2(src + 128);
+        }
       tell(k);
       if (ok) ok = wait(&bars.want, (it - 1) & 1);
     }
