@@ -1,7 +1,8 @@
 """The cache side of one model step, in the order ``ModelWorker.execute`` runs it
 (``runtime/worker/llm_worker/model_worker.py:507-528``): index preparation, copy-on-write of
 diverging prefix blocks, the two handshake switches, and — from inside every attention layer —
-the cache write of that layer's new K / V rows (``models/layers/attention.py:76-85``).
+the cache write of that layer's new K / V rows and the attention over its pages
+(``models/layers/attention.py:76-106``).
 
 It owns nothing but a :class:`StepInputBuilder`; the cache belongs to the model, the events and
 queues to the :class:`KVWorkerHandle`.  One difference from the reference, on purpose: the
@@ -16,7 +17,7 @@ from typing import Dict, List, Optional, Tuple
 import torch
 
 from .kv_worker import KVWorkerHandle
-from .ops import cache_ops
+from .ops import attention_ops, cache_ops
 from .step_inputs import StepIndices, StepInputBuilder
 
 
@@ -70,3 +71,20 @@ class ModelStepCache:
         cache_ops.append_paged_kv_cache(key, value, params.batch_indices, params.positions,
                                         self._layers[layer], params.kv_block_indices,
                                         params.kv_block_indptrs, params.kv_last_block_lens)
+
+    def attend_layer(self, layer: int, query: torch.Tensor, params: StepIndices,
+                     scale: Optional[float] = None) -> torch.Tensor:
+        """The attention of that layer behind its cache write (``attention.py:87-106``): `query`
+        ``[T, num_heads, D]`` or ``[T, num_heads * D]``, this step's tokens in the order of
+        ``params``, over the pages the step's table names.  The prefill requests' tokens (causal
+        among themselves) and the decode requests' go through one call each of
+        :func:`lmserve_b200.ops.paged_attention`.  Returns the output in the shape of `query`;
+        runs on the current stream."""
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        cache, n = self._layers[layer], params.prefill_input_len
+        for rows, pages in ((slice(0, n), params.prefill), (slice(n, n + params.num_decode), params.decode)):
+            if pages is not None:
+                attention_ops.paged_attention(query[rows], cache, pages.kv_indptr, pages.kv_indices,
+                                              pages.kv_last_page_len, qo_indptr=pages.qo_indptr, scale=scale,
+                                              out=out[rows])
+        return out
