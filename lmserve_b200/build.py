@@ -87,14 +87,14 @@ def build_packer(force: bool = False) -> Path:
     """Compiles ``lmserve_b200/_packer.so`` (CPython C API, no CUDA) if it is missing or stale."""
     import sysconfig
     if (not force and PACKER_PATH.exists()
-            and PACKER_PATH.stat().st_mtime >= max(PACKER_SRC.stat().st_mtime, Path(__file__).stat().st_mtime)):
+            and PACKER_PATH.stat().st_mtime >= max(f.stat().st_mtime for f in (PACKER_SRC, PUBLIC_HEADER, Path(__file__)))):
         return PACKER_PATH
     cc = os.environ.get("CC") or shutil.which("gcc") or shutil.which("cc")
     if not cc:
         raise RuntimeError("no C compiler found for the request packer; set CC")
     tmp = PACKER_PATH.with_suffix(".so.tmp")
     cmd = [cc, "-O2", "-fPIC", "-shared", "-Wall", "-I", sysconfig.get_paths()["include"],
-           str(PACKER_SRC), "-o", str(tmp)]
+           str(PACKER_SRC), "-o", str(tmp), "-lm"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"compiling the request packer failed:\n{res.stdout}\n{res.stderr}")

@@ -373,7 +373,8 @@ int attention_params(const lms_attention_args* a, AttentionParams* out, bool* em
       a->num_kv_heads <= 0 || a->num_heads % a->num_kv_heads != 0 || a->head_dim <= 0 ||
       a->block_size <= 0 || a->block_size > (1 << 20) || (a->dtype != 0 && a->dtype != 1) ||
       !(a->scale >= -1e30 && a->scale <= 1e30) ||
-      (a->num_kv_indices + 1) * ((a->block_size + 15) / 16) > kMax ||  // 16-key units of all pages
+      (a->num_kv_indices + 1) * (a->block_size + 16) > kMax ||  // keys, and 16-key units, of all pages
+      (a->num_prefix_indices + 1) * (a->block_size + 16) > kMax ||
       a->num_tokens * (a->num_heads / a->num_kv_heads) > kMax)         // rows of a key head
     return LMS_ERR_RANGE;
   if (a->head_dim % 8 != 0 || a->head_dim > 256) return LMS_ERR_UNSUPPORTED;

@@ -11,10 +11,17 @@
  * straight into a caller-provided buffer (the pinned staging memory).  The requests are any
  * objects with the InferInput attributes of proto/worker.proto:40-47; block_ids and input_ids are
  * any sequences of integers.  Sorting stays with the caller (list.sort, as the reference does).
+ *
+ * The other small helpers of the Python layer live here too: flattening of block maps, calls of
+ * write plans, and the argument checks of the attention-layer calls.
  */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
+#include <math.h>
 #include <stdint.h>
+#include <string.h>
+
+#include "../../include/lmserve_kv.h"
 
 /* Attribute names, interned once at module start-up (a lookup by C string builds a new str
  * object per call). */
@@ -279,53 +286,334 @@ static PyObject* call_plan(PyObject* self, PyObject* const* args, Py_ssize_t nar
   return PyLong_FromLong((long)run(plan, stream));
 }
 
-/* call_words(fn_address, stream, words) -> status
+/* ---- calls of the attention layer ---------------------------------------------------------
  *
- * Calls an `int fn(const void* args, void* stream)` entry point whose `args` is a structure of
- * 8-byte fields (lms_attention_args), built here on the stack from the sequence `words`: an int is
- * stored as a 64-bit integer or address, a float as a double, None as NULL.  With stream = None
- * the entry point is `int64_t fn(const void* args)` (lms_attention_workspace_bytes). */
-#define CALL_WORDS_MAX 64
-typedef int64_t (*size_fn)(const void*);
+ * A layer of a decode step makes one head-norm call and one attention call, each with five to
+ * twelve tensors, and reading what has to be checked of them is most of what a small call costs on
+ * the host.  The two functions below read every attribute once, through the tensors' own Python
+ * attributes, check it, fill the argument structure of the C entry point and call it.  They return
+ * the entry point's status, or None where an argument is not one they take: the Python caller then
+ * says what is wrong with it (or brings it into shape and calls again). */
+#define FACTS_MAX_DIM 6
+typedef struct {
+  PyObject* dtype; /* borrowed: compared by identity, torch's dtypes live for ever */
+  int64_t device;  /* -1 on the host */
+  int64_t ptr;
+  int dim;
+  int64_t size[FACTS_MAX_DIM], stride[FACTS_MAX_DIM]; /* in elements */
+} facts;
 
-static PyObject* call_words(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
-  (void)self;
-  if (nargs != 3 || !(PyTuple_Check(args[2]) || PyList_Check(args[2]))) {
-    PyErr_SetString(PyExc_TypeError, "call_words(fn_address, stream, words)");
-    return NULL;
-  }
-  const Py_ssize_t n = PySequence_Fast_GET_SIZE(args[2]);
-  PyObject** items = PySequence_Fast_ITEMS(args[2]);
-  uint64_t words[CALL_WORDS_MAX];
-  if (n > CALL_WORDS_MAX) {
-    PyErr_SetString(PyExc_ValueError, "call_words: too many words");
-    return NULL;
-  }
-  void* fn = PyLong_AsVoidPtr(args[0]);
-  void* stream = args[1] == Py_None ? NULL : PyLong_AsVoidPtr(args[1]);
-  for (Py_ssize_t i = 0; i < n && !PyErr_Occurred(); ++i) {
-    if (items[i] == Py_None) {
-      words[i] = 0;
-    } else if (PyFloat_Check(items[i])) {
-      const double d = PyFloat_AS_DOUBLE(items[i]);
-      memcpy(&words[i], &d, sizeof(d));
-    } else {
-      words[i] = (uint64_t)(uintptr_t)PyLong_AsVoidPtr(items[i]); /* signed or unsigned 64 bits */
+static PyObject *s_dtype, *s_get_device, *s_data_ptr, *s_shape, *s_stride, *s_new_empty;
+
+static int int_of(PyObject* v, int64_t* out) { /* takes the reference */
+  if (!v) return -1;
+  *out = PyLong_AsLongLong(v);
+  Py_DECREF(v);
+  return *out == -1 && PyErr_Occurred() ? -1 : 0;
+}
+
+static int ints_of(PyObject* v, int64_t* out, int* n) { /* takes the reference */
+  if (!v) return -1;
+  int rc = -1;
+  if (PyTuple_Check(v) && PyTuple_GET_SIZE(v) <= FACTS_MAX_DIM) {
+    *n = (int)PyTuple_GET_SIZE(v);
+    rc = 0;
+    for (int i = 0; i < *n && rc == 0; ++i) {
+      out[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(v, i));
+      if (out[i] == -1 && PyErr_Occurred()) rc = -1;
     }
   }
-  if (PyErr_Occurred()) return NULL;
-  if (fn == NULL) {
-    PyErr_SetString(PyExc_ValueError, "call_words: NULL function address");
+  Py_DECREF(v);
+  return rc;
+}
+
+/* 0, or -1 for anything that is not a tensor of at most FACTS_MAX_DIM dimensions */
+static int facts_of(PyObject* t, facts* f) {
+  int n = 0;
+  PyObject* d = PyObject_GetAttr(t, s_dtype);
+  if (!d) return -1;
+  f->dtype = d;
+  Py_DECREF(d);
+  if (int_of(PyObject_CallMethodNoArgs(t, s_get_device), &f->device)) return -1;
+  if (f->device < 0) { /* nothing on the host is taken */
+    f->dim = -1;
+    return 0;
+  }
+  if (int_of(PyObject_CallMethodNoArgs(t, s_data_ptr), &f->ptr)) return -1;
+  if (ints_of(PyObject_GetAttr(t, s_shape), f->size, &f->dim)) return -1;
+  if (ints_of(PyObject_CallMethodNoArgs(t, s_stride), f->stride, &n) || n != f->dim) return -1;
+  return 0;
+}
+
+static int is_vector(const facts* f, PyObject* dtype, int64_t device, int64_t n) { /* n < 0: any length */
+  return f->dim == 1 && f->dtype == dtype && f->device == device && (n < 0 || f->size[0] == n) &&
+         (f->size[0] <= 1 || f->stride[0] == 1);
+}
+
+#define AS_PTR(x) ((void*)(uintptr_t)(x))
+
+/* The dtype objects, given once by the Python side. */
+static PyObject *dt_f16, *dt_bf16, *dt_i32, *dt_i64, *dt_f32;
+
+static PyObject* set_dtypes(PyObject* self, PyObject* args) {
+  (void)self;
+  PyObject *a, *b, *c, *d, *e;
+  if (!PyArg_ParseTuple(args, "OOOOO", &a, &b, &c, &d, &e)) return NULL;
+  dt_f16 = Py_NewRef(a);
+  dt_bf16 = Py_NewRef(b);
+  dt_i32 = Py_NewRef(c);
+  dt_i64 = Py_NewRef(d);
+  dt_f32 = Py_NewRef(e);
+  Py_RETURN_NONE;
+}
+
+static PyObject* not_taken(void) {
+  PyErr_Clear();
+  Py_RETURN_NONE;
+}
+
+/* attention(size_fn, run_fn, stream, device, query, k_cache, v_cache | None, kv_indptr, kv_indices,
+ *           kv_last, qo_indptr | None, prefix_indptr | None, prefix_indices, prefix_last,
+ *           group_indptr | None, scale | None, causal, out, lse | None) -> status | None
+ *
+ * v_cache None: k_cache is the interleaved [num_pages, 2, page_size, H, D]. */
+typedef int64_t (*attention_size_fn)(const lms_attention_args*);
+typedef int (*attention_run_fn)(const lms_attention_args*, void*);
+
+static PyObject* attention(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (nargs != 19 || dt_i32 == NULL) {
+    PyErr_SetString(PyExc_TypeError, "attention() takes 19 arguments, after set_dtypes()");
     return NULL;
   }
-  if (args[1] == Py_None) {
-    size_fn size;
-    memcpy(&size, &fn, sizeof(size));
-    return PyLong_FromLongLong((long long)size(words));
+  void* size_ptr = PyLong_AsVoidPtr(args[0]);
+  void* run_ptr = PyLong_AsVoidPtr(args[1]);
+  void* stream = PyLong_AsVoidPtr(args[2]);
+  const int64_t device = PyLong_AsLongLong(args[3]);
+  if (PyErr_Occurred()) return NULL;
+  if (!size_ptr || !run_ptr) {
+    PyErr_SetString(PyExc_ValueError, "attention: NULL function address");
+    return NULL;
   }
-  plan_run_fn run;
-  memcpy(&run, &fn, sizeof(run));
-  return PyLong_FromLong((long)run(words, stream));
+  facts q, k, v, out, x;
+  lms_attention_args a;
+  memset(&a, 0, sizeof(a));
+  if (device < 0 || facts_of(args[4], &q) || facts_of(args[5], &k)) return not_taken();
+  const int half = k.dtype == dt_f16;
+  if ((!half && k.dtype != dt_bf16) || q.dtype != k.dtype || q.device != device || k.device != device) return not_taken();
+  const int pair = args[6] != Py_None;
+  if (k.dim != (pair ? 4 : 5)) return not_taken();
+  const int at = k.dim - 3;
+  const int64_t BS = k.size[at], H = k.size[at + 1], D = k.size[at + 2];
+  if (k.stride[at] != H * D || k.stride[at + 1] != D || k.stride[at + 2] != 1 || H <= 0 || D <= 0) return not_taken();
+  a.key_cache = AS_PTR(k.ptr);
+  if (pair) {
+    if (facts_of(args[6], &v) || v.dtype != k.dtype || v.device != device || v.dim != 4 ||
+        memcmp(v.size, k.size, 4 * sizeof(int64_t)) || memcmp(v.stride, k.stride, 4 * sizeof(int64_t)))
+      return not_taken();
+    a.value_cache = AS_PTR(v.ptr);
+  } else {
+    if (k.size[1] != 2) return not_taken();
+    a.value_cache = AS_PTR(k.ptr + k.stride[1] * 2);
+  }
+  int64_t HQ;
+  const int64_t T = q.dim > 0 ? q.size[0] : 0;
+  if (q.dim == 3) {
+    HQ = q.size[1];
+    if (q.size[2] != D || (T && (q.stride[2] != 1 || (HQ != 1 && q.stride[1] != D)))) return not_taken();
+  } else if (q.dim == 2) {
+    HQ = q.size[1] / D;
+    if (HQ * D != q.size[1] || (T && q.stride[1] != 1)) return not_taken();
+  } else {
+    return not_taken();
+  }
+  if (HQ <= 0 || HQ % H) return not_taken();
+  if (facts_of(args[17], &out) || out.dtype != q.dtype || out.device != device || out.dim != q.dim ||
+      memcmp(out.size, q.size, (size_t)q.dim * sizeof(int64_t)) ||
+      (T && (out.stride[q.dim - 1] != 1 || (q.dim == 3 && HQ != 1 && out.stride[1] != D))))
+    return not_taken();
+  if (facts_of(args[7], &x) || !is_vector(&x, dt_i32, device, -1) || x.size[0] < 1) return not_taken();
+  const int64_t B = x.size[0] - 1;
+  a.kv_indptr = AS_PTR(x.ptr);
+  if (facts_of(args[8], &x) || !is_vector(&x, dt_i32, device, -1)) return not_taken();
+  a.kv_indices = AS_PTR(x.ptr);
+  a.num_kv_indices = x.size[0];
+  if (facts_of(args[9], &x) || !is_vector(&x, dt_i32, device, B)) return not_taken();
+  a.kv_last_page_len = AS_PTR(x.ptr);
+  if (args[10] != Py_None) {
+    if (facts_of(args[10], &x) || !is_vector(&x, dt_i32, device, B + 1)) return not_taken();
+    a.qo_indptr = AS_PTR(x.ptr);
+  } else if (T != B) {
+    return not_taken();
+  }
+  if (args[11] != Py_None) {
+    if (facts_of(args[11], &x) || !is_vector(&x, dt_i32, device, -1) || x.size[0] < 1) return not_taken();
+    a.num_groups = x.size[0] - 1;
+    a.prefix_indptr = AS_PTR(x.ptr);
+    if (facts_of(args[12], &x) || !is_vector(&x, dt_i32, device, -1)) return not_taken();
+    a.prefix_indices = AS_PTR(x.ptr);
+    a.num_prefix_indices = x.size[0];
+    if (facts_of(args[13], &x) || !is_vector(&x, dt_i32, device, a.num_groups)) return not_taken();
+    a.prefix_last_page_len = AS_PTR(x.ptr);
+    if (args[14] != Py_None) {
+      if (facts_of(args[14], &x) || !is_vector(&x, dt_i32, device, a.num_groups + 1)) return not_taken();
+      a.group_indptr = AS_PTR(x.ptr);
+    } else if (a.num_groups != 1) {
+      return not_taken();
+    }
+  }
+  if (args[18] != Py_None) {
+    if (facts_of(args[18], &x) || x.dtype != dt_f32 || x.device != device || x.dim != 2 || x.size[0] != T ||
+        x.size[1] != HQ || (T > 1 && x.stride[0] != HQ) || (T && HQ > 1 && x.stride[1] != 1))
+      return not_taken();
+    a.lse = AS_PTR(x.ptr);
+  }
+  if (args[15] == Py_None) {
+    a.scale = 1.0 / sqrt((double)D);
+  } else {
+    a.scale = PyFloat_AsDouble(args[15]);
+    if (PyErr_Occurred()) return NULL;
+  }
+  a.causal = PyObject_IsTrue(args[16]);
+  if (a.causal < 0) return NULL;
+  if (T == 0 || B == 0) return PyLong_FromLong(0);
+  a.query = AS_PTR(q.ptr);
+  a.out = AS_PTR(out.ptr);
+  a.query_token_stride = T > 1 ? q.stride[0] * 2 : 0; /* the distance to a next token, if there is one */
+  a.out_token_stride = T > 1 ? out.stride[0] * 2 : 0;
+  a.block_stride = k.stride[0] * 2;
+  a.slot_stride = H * D * 2;
+  a.num_tokens = T;
+  a.num_requests = B;
+  a.num_blocks = k.size[0];
+  a.num_heads = HQ;
+  a.num_kv_heads = H;
+  a.head_dim = D;
+  a.block_size = BS;
+  a.dtype = half ? 0 : 1;
+
+  attention_size_fn size;
+  attention_run_fn run;
+  memcpy(&size, &size_ptr, sizeof(size));
+  memcpy(&run, &run_ptr, sizeof(run));
+  const int64_t need = size(&a);
+  if (need < 0) return PyLong_FromLongLong(need);
+  PyObject* workspace = NULL;
+  if (need > 0) {
+    /* taken per call from torch's allocator: ordered by the stream it is used on, and a captured call
+     * keeps its own; `need` is a multiple of 256, the tensor is int32 as kv_indptr is */
+    PyObject* n = PyLong_FromLongLong(need / 4);
+    if (!n) return NULL;
+    workspace = PyObject_CallMethodOneArg(args[7], s_new_empty, n);
+    Py_DECREF(n);
+    int64_t ptr = 0;
+    if (!workspace) return NULL;
+    if (int_of(PyObject_CallMethodNoArgs(workspace, s_data_ptr), &ptr)) {
+      Py_DECREF(workspace);
+      return NULL;
+    }
+    a.workspace = AS_PTR(ptr);
+    a.workspace_bytes = need;
+  }
+  const int rc = run(&a, stream);
+  Py_XDECREF(workspace);
+  return PyLong_FromLong((long)rc);
+}
+
+/* qk_norm(run_fn, stream, device, query, key, value | None, query_weight, key_weight, positions,
+ *         cos_sin_cache, head_dim, kv_cache | None, slots | None, eps, q_out, k_out | None)
+ *         -> status | None
+ *
+ * q_out and k_out are fresh, contiguous and shaped as query and key. */
+typedef int (*qk_norm_run_fn)(const lms_qk_norm_args*, void*);
+
+static PyObject* qk_norm(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (nargs != 16 || dt_i32 == NULL) {
+    PyErr_SetString(PyExc_TypeError, "qk_norm() takes 16 arguments, after set_dtypes()");
+    return NULL;
+  }
+  void* run_ptr = PyLong_AsVoidPtr(args[0]);
+  void* stream = PyLong_AsVoidPtr(args[1]);
+  const int64_t device = PyLong_AsLongLong(args[2]);
+  const int64_t D = PyLong_AsLongLong(args[10]);
+  const double eps = PyFloat_AsDouble(args[13]);
+  if (PyErr_Occurred()) return NULL;
+  if (!run_ptr) {
+    PyErr_SetString(PyExc_ValueError, "qk_norm: NULL function address");
+    return NULL;
+  }
+  facts q, k, x;
+  lms_qk_norm_args a;
+  memset(&a, 0, sizeof(a));
+  if (device < 0 || D <= 0 || facts_of(args[3], &q) || facts_of(args[4], &k)) return not_taken();
+  PyObject* const dtype = q.dtype;
+  if ((dtype != dt_f16 && dtype != dt_bf16) || k.dtype != dtype || q.device != device || k.device != device ||
+      q.dim != 2 || k.dim != 2 || k.size[0] != q.size[0])
+    return not_taken();
+  const int64_t T = q.size[0], heads = q.size[1] / D, kv_heads = k.size[1] / D;
+  if (heads <= 0 || kv_heads <= 0 || heads * D != q.size[1] || kv_heads * D != k.size[1] || q.stride[1] != 1 ||
+      k.stride[1] != 1)
+    return not_taken();
+  if (facts_of(args[6], &x) || !is_vector(&x, dtype, device, D)) return not_taken();
+  a.query_weight = AS_PTR(x.ptr);
+  if (facts_of(args[7], &x) || !is_vector(&x, dtype, device, D)) return not_taken();
+  a.key_weight = AS_PTR(x.ptr);
+  if (facts_of(args[8], &x)) return not_taken();
+  a.positions_are_int64 = x.dtype == dt_i64;
+  if (!is_vector(&x, a.positions_are_int64 ? dt_i64 : dt_i32, device, T)) return not_taken();
+  a.positions = AS_PTR(x.ptr);
+  if (facts_of(args[9], &x) || x.dtype != dtype || x.device != device || x.dim != 2 || x.size[1] != 2 * D ||
+      x.stride[1] != 1)
+    return not_taken();
+  a.cos_sin_cache = AS_PTR(x.ptr);
+  a.cos_sin_row_stride = x.size[0] > 1 ? x.stride[0] * 2 : 0;
+  a.max_position = x.size[0];
+  const int one = T == 1; /* the distance to a next token means nothing */
+  if (args[11] != Py_None) {
+    const int64_t row = kv_heads * D;
+    if (facts_of(args[11], &x) || x.dtype != dtype || x.device != device || x.dim != 5 || x.size[1] != 2 ||
+        x.size[3] != kv_heads || x.size[4] != D)
+      return not_taken();
+    const int64_t NB = x.size[0], BS = x.size[2];
+    if (NB && (x.stride[1] != BS * row || x.stride[2] != row || x.stride[3] != D || x.stride[4] != 1)) return not_taken();
+    a.key_cache = AS_PTR(x.ptr);
+    a.value_cache = AS_PTR(x.ptr + BS * row * 2);
+    a.block_stride = x.stride[0] * 2;
+    a.slot_stride = row * 2;
+    a.block_size = BS;
+    a.num_slots = NB * BS;
+    if (facts_of(args[5], &x) || x.dtype != dtype || x.device != device || x.dim != 2 || x.size[0] != T ||
+        x.size[1] != k.size[1] || x.stride[1] != 1)
+      return not_taken();
+    a.value = AS_PTR(x.ptr);
+    a.value_token_stride = one ? 0 : x.stride[0] * 2;
+    if (facts_of(args[12], &x) || !is_vector(&x, dt_i64, device, T)) return not_taken();
+    a.slot_mapping = AS_PTR(x.ptr);
+  }
+  if (T == 0) return PyLong_FromLong(0);
+  int64_t ptr;
+  if (int_of(PyObject_CallMethodNoArgs(args[14], s_data_ptr), &ptr)) return NULL;
+  a.q_out = AS_PTR(ptr);
+  a.q_out_token_stride = q.size[1] * 2;
+  if (args[15] != Py_None) {
+    if (int_of(PyObject_CallMethodNoArgs(args[15], s_data_ptr), &ptr)) return NULL;
+    a.k_out = AS_PTR(ptr);
+    a.k_out_token_stride = k.size[1] * 2;
+  }
+  a.query = AS_PTR(q.ptr);
+  a.key = AS_PTR(k.ptr);
+  a.query_token_stride = one ? 0 : q.stride[0] * 2;
+  a.key_token_stride = one ? 0 : k.stride[0] * 2;
+  a.eps = eps;
+  a.num_tokens = T;
+  a.num_heads = heads;
+  a.num_kv_heads = kv_heads;
+  a.head_dim = D;
+  a.dtype = dtype == dt_f16 ? 0 : 1;
+  qk_norm_run_fn run;
+  memcpy(&run, &run_ptr, sizeof(run));
+  return PyLong_FromLong((long)run(&a, stream));
 }
 
 static PyMethodDef methods[] = {
@@ -336,8 +624,11 @@ static PyMethodDef methods[] = {
      "prefill_blocks, decode_blocks)"},
     {"call_plan", (PyCFunction)(void (*)(void))call_plan, METH_FASTCALL,
      "call_plan(fn_address, plan_handle, stream) -> status of int fn(plan, stream)"},
-    {"call_words", (PyCFunction)(void (*)(void))call_words, METH_FASTCALL,
-     "call_words(fn_address, stream, words) -> status of int fn(struct of words, stream)"},
+    {"set_dtypes", set_dtypes, METH_VARARGS, "set_dtypes(float16, bfloat16, int32, int64, float32)"},
+    {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL,
+     "attention(...) -> status of lms_paged_attention, or None for arguments it does not take"},
+    {"qk_norm", (PyCFunction)(void (*)(void))qk_norm, METH_FASTCALL,
+     "qk_norm(...) -> status of lms_qk_norm_rope_and_cache, or None for arguments it does not take"},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_packer",
@@ -350,6 +641,13 @@ PyMODINIT_FUNC PyInit__packer(void) {
   s_context_len = PyUnicode_InternFromString("context_len");
   s_block_ids = PyUnicode_InternFromString("block_ids");
   s_input_ids = PyUnicode_InternFromString("input_ids");
+  s_dtype = PyUnicode_InternFromString("dtype");
+  s_get_device = PyUnicode_InternFromString("get_device");
+  s_data_ptr = PyUnicode_InternFromString("data_ptr");
+  s_shape = PyUnicode_InternFromString("shape");
+  s_stride = PyUnicode_InternFromString("stride");
+  s_new_empty = PyUnicode_InternFromString("new_empty");
+  if (!s_dtype || !s_get_device || !s_data_ptr || !s_shape || !s_stride || !s_new_empty) return NULL;
   if (!s_input_len || !s_filled_token_len || !s_context_len || !s_block_ids || !s_input_ids) return NULL;
   return PyModule_Create(&module);
 }

@@ -38,7 +38,7 @@ def _entry_points() -> Tuple[int, int]:
 
 def _refuse(query, paged_kv_cache, lists, qo_indptr, group_indptr, out):
     """Names what is wrong with the arguments of an attention call."""
-    if type(paged_kv_cache) is torch.Tensor:
+    if isinstance(paged_kv_cache, torch.Tensor):
         k_cache = v_cache = paged_kv_cache
         if k_cache.dim() != 5 or k_cache.shape[1] != 2:
             raise ValueError("paged_kv_cache must be [num_pages, 2, page_size, H, D]")
@@ -99,110 +99,33 @@ def _check_index(name: str, t: torch.Tensor, dev: torch.device) -> None:
         raise ValueError(f"{name} must be a contiguous vector on the cache's device")
 
 
-def _attention(query, paged_kv_cache: Cache, lists, group_indptr, qo_indptr, scale, causal, return_lse, out):
-    # A layer of a decode step makes this call once, and the host's part of it is most of what a
-    # small one costs: every attribute is read once, all checks are one expression, and only a call
-    # that fails it is looked at again, to say what is wrong.
-    _, _, (kv_indptr, kv_indices, kv_last) = lists[0]
-    if type(paged_kv_cache) is torch.Tensor:
-        k_cache = v_cache = paged_kv_cache
-        cshape, cstride = k_cache.shape, k_cache.stride()
-        ok = len(cshape) == 5 and cshape[1] == 2
+def _attention(query, paged_kv_cache: Cache, own, prefix, group_indptr, qo_indptr, scale, causal, return_lse, out):
+    idx = query.get_device()
+    if idx >= 0 and idx != _current_device():
+        with torch.cuda.device(idx):
+            return _attention(query, paged_kv_cache, own, prefix, group_indptr, qo_indptr, scale, causal, return_lse, out)
+    if isinstance(paged_kv_cache, torch.Tensor):
+        k_cache, v_cache = paged_kv_cache, None
     else:
         k_cache, v_cache = paged_kv_cache
-        cshape, cstride = k_cache.shape, k_cache.stride()
-        ok = (len(cshape) == 4 and cshape == v_cache.shape and cstride == v_cache.stride()
-              and v_cache.dtype is k_cache.dtype and v_cache.get_device() == k_cache.get_device())
-    dtype, idx = k_cache.dtype, k_cache.get_device()
-    qshape, qstride = query.shape, query.stride()
-    code = _DTYPE_CODE.get(dtype)
-    if ok and idx >= 0 and code is not None and query.dtype is dtype and query.get_device() == idx:
-        H, D = cshape[-2], cshape[-1]
-        HD = H * D
-        nk = kv_indices.shape[0] if kv_indices.dim() == 1 else -1
-        B = kv_indptr.shape[0] - 1 if kv_indptr.dim() == 1 else -1
-        T = qshape[0] if qshape else 0
-        if len(qshape) == 3:
-            HQ = qshape[1]
-            ok = qshape[2] == D and (T == 0 or (qstride[2] == 1 and (HQ == 1 or qstride[1] == D)))
-        elif len(qshape) == 2 and D:
-            HQ = qshape[1] // D
-            ok = HQ * D == qshape[1] and (T == 0 or qstride[1] == 1)
-        else:
-            HQ, ok = 0, False
-        ok = (ok and HQ > 0 and H > 0 and HQ % H == 0 and cstride[-3:] == (HD, D, 1) and B >= 0 and nk >= 0
-              and kv_indptr.dtype is _I32 and kv_indices.dtype is _I32 and kv_last.dtype is _I32
-              and kv_indptr.get_device() == idx and kv_indices.get_device() == idx and kv_last.get_device() == idx
-              and kv_indptr.is_contiguous() and kv_indices.is_contiguous() and kv_last.is_contiguous()
-              and kv_last.shape == (B,))
-    else:
-        ok = False
-    qo = pp = pi = pe = gp = None
-    n_prefix = G = 0
-    if ok:
-        if qo_indptr is None:
-            ok = T == B
-        else:
-            ok = (qo_indptr.shape == (B + 1,) and qo_indptr.dtype is _I32 and qo_indptr.get_device() == idx
-                  and qo_indptr.is_contiguous())
-            qo = qo_indptr.data_ptr()
-    if ok and len(lists) == 2:
-        _, _, (indptr, indices, last) = lists[1]
-        n_prefix = indices.shape[0] if indices.dim() == 1 else -1
-        G = indptr.shape[0] - 1 if indptr.dim() == 1 else -1
-        ok = (G >= 0 and n_prefix >= 0 and last.shape == (G,)
-              and indptr.dtype is _I32 and indices.dtype is _I32 and last.dtype is _I32
-              and indptr.get_device() == idx and indices.get_device() == idx and last.get_device() == idx
-              and indptr.is_contiguous() and indices.is_contiguous() and last.is_contiguous())
-        pp, pi, pe = indptr.data_ptr(), indices.data_ptr(), last.data_ptr()
-        if group_indptr is None:
-            ok = ok and G == 1
-        else:
-            ok = (ok and group_indptr.shape == (G + 1,) and group_indptr.dtype is _I32
-                  and group_indptr.get_device() == idx and group_indptr.is_contiguous())
-            gp = group_indptr.data_ptr()
-    if not ok:
-        _refuse(query, paged_kv_cache, lists, qo_indptr, group_indptr, None)
-    if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)
-        o_tok = HQ * D
-    else:
-        ostride = out.stride()
-        if (out.shape != qshape or out.dtype is not dtype or out.get_device() != idx
-                or T and (ostride[-1] != 1 or (len(qshape) == 3 and HQ > 1 and ostride[1] != D))):
-            _refuse(query, paged_kv_cache, lists, qo_indptr, group_indptr, out)
-        o_tok = ostride[0]
-    lse = torch.empty((T, HQ), dtype=torch.float32, device=query.device) if return_lse else None
-    if T and B:
-        kptr = k_cache.data_ptr()
-        words = [query.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None, kptr,
-                 kptr + cstride[1] * 2 if v_cache is k_cache else v_cache.data_ptr(),
-                 qstride[0] * 2 if T > 1 else 0, o_tok * 2 if T > 1 else 0, cstride[0] * 2, HD * 2,
-                 kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last.data_ptr(), nk, qo, pp, pi, pe, n_prefix, gp,
-                 T, B, G, cshape[0], HQ, H, D, cshape[-3], code, 1 if causal else 0,
-                 D ** -0.5 if scale is None else float(scale), None, 0]
-        size_of, run = _entries or _entry_points()
-        if idx != _current_device():
-            with torch.cuda.device(idx):
-                _enqueue(size_of, run, words, kv_indptr, idx)
-        else:
-            _enqueue(size_of, run, words, kv_indptr, idx)
-    return (out, lse) if return_lse else out
-
-
-def _enqueue(size_of, run, words, like, idx):
-    need = _packer.call_words(size_of, None, words)
-    if need > 0:
-        # taken per call from the caching allocator: ordered by the stream it is used on, and a
-        # captured call keeps its own
-        workspace = like.new_empty(need >> 2)  # int32; `need` is a multiple of 256
-        words[-2] = workspace.data_ptr()
-        words[-1] = need
-    elif need:
-        _lib.check(need)
-    rc = _packer.call_words(run, _raw_stream_of(idx), words)
+    result = torch.empty_like(query, memory_format=torch.contiguous_format) if out is None else out
+    lse = None
+    if return_lse:
+        shape = query.shape
+        heads = shape[1] if len(shape) == 3 else shape[1] // max(1, k_cache.shape[-1]) if len(shape) == 2 else 0
+        lse = torch.empty((shape[0] if shape else 0, heads), dtype=torch.float32, device=query.device)
+    size_of, run = _entries or _entry_points()
+    # all checks of the tensors are made there (csrc/packer.c)
+    rc = _packer.attention(size_of, run, _raw_stream_of(idx) if idx >= 0 else 0, idx, query, k_cache, v_cache, *own,
+                           qo_indptr, *prefix, group_indptr, scale, causal, result, lse)
     if rc:
         _lib.check(rc)
+    elif rc is None:
+        lists = [("kv_", "request", own)]
+        if prefix[0] is not None:
+            lists.append(("prefix_", "group", prefix))
+        _refuse(query, paged_kv_cache, lists, qo_indptr, group_indptr, out)
+    return (result, lse) if return_lse else result
 
 
 def paged_attention(query: torch.Tensor, paged_kv_cache: Cache, kv_indptr: torch.Tensor,
@@ -230,8 +153,8 @@ def paged_attention(query: torch.Tensor, paged_kv_cache: Cache, kv_indptr: torch
 
     Head dims up to 256 that are multiples of 8.
     """
-    return _attention(query, paged_kv_cache, (("kv_", "request", (kv_indptr, kv_indices, kv_last_page_len)),),
-                      None, qo_indptr, scale, causal, return_lse, out)
+    return _attention(query, paged_kv_cache, (kv_indptr, kv_indices, kv_last_page_len), (None, None, None), None,
+                      qo_indptr, scale, causal, return_lse, out)
 
 
 def shared_prefix_attention(query: torch.Tensor, paged_kv_cache: Cache,
@@ -252,7 +175,6 @@ def shared_prefix_attention(query: torch.Tensor, paged_kv_cache: Cache,
     concerns the own keys only.  A prefix may be empty, a group too, and a request outside every
     group has no prefix.  The other arguments are those of :func:`paged_attention`.
     """
-    return _attention(query, paged_kv_cache,
-                      (("kv_", "request", (kv_indptr, kv_indices, kv_last_page_len)),
-                       ("prefix_", "group", (prefix_indptr, prefix_indices, prefix_last_page_len))),
-                      group_indptr, qo_indptr, scale, causal, return_lse, out)
+    return _attention(query, paged_kv_cache, (kv_indptr, kv_indices, kv_last_page_len),
+                      (prefix_indptr, prefix_indices, prefix_last_page_len), group_indptr,
+                      qo_indptr, scale, causal, return_lse, out)

@@ -42,6 +42,7 @@ except AttributeError:  # pragma: no cover - older / newer torch
 # The same two lookups for callers that hold a device index (CUDA is initialised by then).
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream_of = _raw_stream or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_packer.set_dtypes(torch.float16, torch.bfloat16, torch.int32, torch.int64, torch.float32)
 
 
 # Host address of a registered host pool -> the address the GPU uses for the same memory

@@ -196,67 +196,33 @@ def _refuse_qk_norm(query, key, value, query_weight, key_weight, positions, cos_
 
 def _qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps,
              kv_cache, slot_mapping, return_key):
-    # One such call a layer: attributes are read once, all checks are one expression, and only a
-    # call that fails it is looked at again, to say what is wrong.
-    for t in (query, key, query_weight, key_weight, positions, cos_sin_cache):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"expected a torch.Tensor, got {type(t).__name__}")
-    dtype, idx = query.dtype, query.get_device()
-    code = _DTYPE_CODE.get(dtype)
-    qshape, kshape, cshape = query.shape, key.shape, cos_sin_cache.shape
-    slots = slot_mapping
-    ok = (idx >= 0 and code is not None and len(qshape) == 2 and len(kshape) == 2 and len(cshape) == 2 and head_dim > 0
-          and key.dtype is dtype and cos_sin_cache.dtype is dtype and query_weight.dtype is dtype
-          and key_weight.dtype is dtype and key.get_device() == idx and cos_sin_cache.get_device() == idx
-          and query_weight.get_device() == idx and key_weight.get_device() == idx and positions.get_device() == idx)
-    if ok:
-        T = qshape[0]
-        qstride, kstride, cstride, pdtype = query.stride(), key.stride(), cos_sin_cache.stride(), positions.dtype
-        heads, kv_heads = qshape[1] // head_dim, kshape[1] // head_dim
-        ok = (kshape[0] == T and heads > 0 and kv_heads > 0 and heads * head_dim == qshape[1]
-              and kv_heads * head_dim == kshape[1] and cshape[1] == 2 * head_dim
-              and qstride[1] == 1 and kstride[1] == 1 and cstride[1] == 1
-              and query_weight.shape == key_weight.shape == (head_dim,) and query_weight.is_contiguous()
-              and key_weight.is_contiguous() and positions.shape == (T,)
-              and (pdtype is torch.int32 or pdtype is torch.int64))
-    if ok and kv_cache is not None:
-        lshape, lstride, vstride = kv_cache.shape, kv_cache.stride(), value.stride()
-        row = kv_heads * head_dim
-        if slots.dtype is not torch.int64 or slots.get_device() != idx or not slots.is_contiguous():
-            slots = _slots_i64(slot_mapping, query.device)
-        ok = (len(lshape) == 5 and lshape[1] == 2 and lshape[3] == kv_heads and lshape[4] == head_dim
-              and (lshape[0] == 0 or lstride[1:] == (lshape[2] * row, row, head_dim, 1))
-              and kv_cache.dtype is dtype and value.dtype is dtype and kv_cache.get_device() == idx
-              and value.get_device() == idx and value.shape == kshape and vstride[1] == 1 and slots.shape == (T,))
-    if not ok:
-        _refuse_qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cache, head_dim, kv_cache, slots)
+    idx = query.get_device()
+    if idx >= 0 and idx != _current_device():
+        with torch.cuda.device(idx):
+            return _qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps,
+                            kv_cache, slot_mapping, return_key)
+    global _qk_norm_entry
+    if _qk_norm_entry is None:
+        _qk_norm_entry = ctypes.cast(_lib.lib().lms_qk_norm_rope_and_cache, ctypes.c_void_p).value
+    stream = _raw_stream_of(idx) if idx >= 0 else 0
     q_out = torch.empty_like(query, memory_format=torch.contiguous_format)
     k_out = torch.empty_like(key, memory_format=torch.contiguous_format) if return_key else None
-    if T:
-        if not positions.is_contiguous():
-            positions = positions.contiguous()
-        one = T == 1  # the distance to a next token means nothing
-        words = [query.data_ptr(), key.data_ptr(), None, 0 if one else qstride[0] * 2, 0 if one else kstride[0] * 2, 0,
-                 query_weight.data_ptr(), key_weight.data_ptr(), float(eps), positions.data_ptr(),
-                 1 if pdtype is torch.int64 else 0, cos_sin_cache.data_ptr(), cstride[0] * 2, q_out.data_ptr(),
-                 qshape[1] * 2, k_out.data_ptr() if return_key else None, kshape[1] * 2,
-                 None, None, 0, 0, None, T, heads, kv_heads, head_dim, code, 0, 0, cshape[0]]
-        if kv_cache is not None:
-            base = kv_cache.data_ptr()
-            words[2] = value.data_ptr()
-            words[5] = 0 if one else vstride[0] * 2
-            words[17:22] = base, base + lshape[2] * row * 2, lstride[0] * 2, row * 2, slots.data_ptr()
-            words[27:29] = lshape[2], lshape[0] * lshape[2]
-        global _qk_norm_entry
-        if _qk_norm_entry is None:
-            _qk_norm_entry = ctypes.cast(_lib.lib().lms_qk_norm_rope_and_cache, ctypes.c_void_p).value
-        if idx != _current_device():
-            with torch.cuda.device(idx):
-                rc = _packer.call_words(_qk_norm_entry, _raw_stream_of(idx), words)
-        else:
-            rc = _packer.call_words(_qk_norm_entry, _raw_stream_of(idx), words)
-        if rc:
-            _lib.check(rc)
+    # all checks of the tensors are made there (csrc/packer.c)
+    rc = _packer.qk_norm(_qk_norm_entry, stream, idx, query, key, value, query_weight, key_weight, positions,
+                         cos_sin_cache, head_dim, kv_cache, slot_mapping, eps, q_out, k_out)
+    if rc is None:  # index arrays as the other cache operators take them, or something is wrong
+        slots = slot_mapping
+        if idx >= 0:
+            if isinstance(slots, torch.Tensor):
+                slots = _slots_i64(slots, query.device)
+            if isinstance(positions, torch.Tensor):
+                positions = positions.contiguous()
+            rc = _packer.qk_norm(_qk_norm_entry, stream, idx, query, key, value, query_weight, key_weight, positions,
+                                 cos_sin_cache, head_dim, kv_cache, slots, eps, q_out, k_out)
+        if rc is None:
+            _refuse_qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cache, head_dim, kv_cache, slots)
+    if rc:
+        _lib.check(rc)
     return (q_out, k_out) if return_key else q_out
 
 

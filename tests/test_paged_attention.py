@@ -472,7 +472,8 @@ def test_argument_errors_of_the_c_entry():
     assert L.lms_paged_attention(None, None) == _lib.LMS_ERR_NULL
     assert f(T=0, B=0) == _lib.LMS_OK and L.lms_attention_workspace_bytes(c_args(T=0, B=0)) == 0
     for kw in (dict(T=-1), dict(T=3), dict(HQ=7), dict(H=0), dict(BS=0), dict(dt=2), dict(NB=-1), dict(nk=-1),
-               dict(scale=math.inf), dict(scale=math.nan), dict(G=-1)):
+               dict(scale=math.inf), dict(scale=math.nan), dict(G=-1), dict(nk=2 ** 27), dict(G=1, np=2 ** 27),
+               dict(T=2 ** 30, B=2 ** 30)):
         assert f(**kw) == _lib.LMS_ERR_RANGE, kw
         assert L.lms_attention_workspace_bytes(c_args(**kw)) == _lib.LMS_ERR_RANGE, kw
     for kw in (dict(D=100), dict(D=264)):
