@@ -325,11 +325,11 @@ typedef struct lms_qk_norm_args {
 int lms_qk_norm_rope_and_cache(const lms_qk_norm_args* args, void* stream);
 
 /*
- * Attention of a batch over its pages of one layer's cache - the call of
- *   prefill_wrapper.run / decode_wrapper.run   runtime/worker/llm_worker/models/layers/attention.py:87-106
- * (flashinfer's paged wrappers) on the index arrays lms_build_step_indices leaves on the device,
- * without a planning step: every launch derives its work from those arrays on the device, so a
- * captured call follows their contents from replay to replay.
+ * Attention of a batch over its pages of one layer's cache - the step behind the cache write of
+ *   runtime/worker/llm_worker/models/layers/attention.py:87-106
+ * on the index arrays lms_build_step_indices leaves on the device.  There is no planning step: every
+ * launch derives its work from those arrays on the device, so a captured call follows their contents
+ * from replay to replay.
  *
  * query [num_tokens, num_heads, head_dim] (token stride in bytes, heads dense), out likewise, lse
  * float [num_tokens, num_heads] or NULL.  Request b owns the pages

@@ -1,8 +1,7 @@
 """Attention of a batch over its pages of one layer's cache.
 
-``paged_attention`` is the call LMServe's attention layer makes after the cache write
-(``models/layers/attention.py:87-106``, flashinfer's paged prefill and decode wrappers), on the
-index arrays that :class:`lmserve_b200.step_inputs.StepInputBuilder` leaves on the device:
+``paged_attention`` is the step behind the cache write in LMServe's attention layer
+(``models/layers/attention.py:87-106``), on the index arrays that :class:`lmserve_b200.step_inputs.StepInputBuilder` leaves on the device:
 ``params.prefill`` and ``params.decode`` hold its arguments.  There is nothing to plan: the
 kernels read the lengths from those arrays, so a call captured into a CUDA graph follows their
 contents from replay to replay.  ``shared_prefix_attention`` is the same attention for requests
