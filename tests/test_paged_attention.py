@@ -500,3 +500,93 @@ def test_the_oracle_on_a_case_done_by_hand():
     own = (torch.tensor([0, 1]), torch.tensor([0]), torch.tensor([2]))
     out, _, lse, _ = attention_oracle.paged_attention(q, cache[:, 0], cache[:, 1], own, scale=1.0)
     assert torch.allclose(out, torch.full_like(out, 7.0)) and abs(lse.item() - math.log(4.0)) < 1e-6
+
+
+def drawn(seed):
+    """A random call: geometry, lengths (zeros and single keys often), groups, stray requests."""
+    import random
+    r = random.Random(seed)
+    D = r.choice([64, 64, 128, 128, 128, 8, 40, 96, 256])
+    H = r.choice([1, 1, 2, 3, 4, 5, 8, 9])
+    G = r.choice([1, 2, 3, 4, 7, 8, 9, 16, 17, 33])
+    B = r.choice([1, 2, 3, 9, 33, 70])
+    most = r.choice([1, 20, 140, 600]) if B < 40 else r.choice([1, 20, 60])
+    length = lambda: r.choice([0, 1, r.randint(0, most), r.randint(0, most), r.randint(0, most)])
+    lengths = [length() for _ in range(B)]
+    new = None
+    if r.random() < 0.6:
+        new = [r.choice([0, 1, r.randint(0, 6), r.randint(0, max(1, min(most, 2 * n)))]) for n in lengths]
+        if sum(new) > 700:
+            new = [min(n, 3) for n in new]
+        if sum(new) == 0:
+            new[0] = 1
+    prefix = groups = None
+    if r.random() < 0.5:
+        n = r.choice([1, 1, 2, 4])
+        prefix = [length() for _ in range(n)]
+        if n > 1 or r.random() < 0.5:
+            groups = sorted(r.randint(0, B) for _ in range(n + 1))
+    c = case(lengths, new, HQ=H * G, H=H, D=D, BS=r.choice([1, 5, 8, 12, 16, 16, 16, 24, 32, 64, 128, 256]),
+             dtype=r.choice([HF, BF]), prefix=prefix, groups=groups, seed=seed, spread=r.choice([0.5, 2.0, 6.0]))
+    return c, dict(causal=r.random() < 0.8)
+
+
+@gpu
+@pytest.mark.parametrize("seed", range(40))
+def test_random_calls(seed):
+    c, kw = drawn(seed)
+    check(c, **kw)
+
+
+@gpu
+def test_thousands_of_requests():
+    """More requests than a warp's, a block's or an SM count's worth, single tokens and a few each."""
+    lengths = [i % 7 for i in range(5000)]
+    c = case(lengths, HQ=4, H=2, D=64, dtype=HF)
+    out, lse = call(c, return_lse=True)
+    some = torch.arange(0, 5000, 41)
+    picked = dict(c, q=c["q"][some], own=(c["own"][0], c["own"][1], c["own"][2]))
+    lists = [c["own"][1][c["own"][0][b]:c["own"][0][b + 1]].tolist() for b in some]
+    picked["own"] = (torch.tensor([0, *torch.tensor([len(x) for x in lists]).cumsum(0)], dtype=torch.int32),
+                     torch.tensor(sum(lists, []), dtype=torch.int32), c["own"][2][some])
+    compare(out[some.to(DEV)], lse[some.to(DEV)], exact(picked))
+    new = [1 + i % 3 for i in range(3000)]
+    c = case([n + i % 5 for i, n in enumerate(new)], new, HQ=4, H=2, D=64, dtype=HF)
+    out, lse = call(c, return_lse=True)
+    first = c["qo"].tolist()
+    some = list(range(0, 3000, 61))
+    rows = [t for b in some for t in range(first[b], first[b + 1])]
+    lists = [c["own"][1][c["own"][0][b]:c["own"][0][b + 1]].tolist() for b in some]
+    picked = dict(c, q=c["q"][rows], qo=torch.tensor([0, *torch.tensor([new[b] for b in some]).cumsum(0)], dtype=torch.int32),
+                  own=(torch.tensor([0, *torch.tensor([len(x) for x in lists]).cumsum(0)], dtype=torch.int32),
+                       torch.tensor(sum(lists, []), dtype=torch.int32), c["own"][2][some]))
+    compare(out[rows], lse[rows], exact(picked))
+
+
+@gpu
+def test_the_first_call_may_be_captured():
+    """In a fresh process: per-device set-up, then a capture with no call before it."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch, sys
+sys.path.insert(0, 'tests')
+from lmserve_b200 import _lib
+from lmserve_b200.ops import paged_attention
+from test_paged_attention import case, exact, compare
+torch.cuda.init(); torch.zeros(1, device='cuda')
+_lib.check(_lib.lib().lms_init_device())
+for new in (None, [30, 1, 200]):
+    c = case([100, 7, 300], new)
+    d = [t.cuda() for t in (c['q'], c['cache'], *c['own'])]
+    qo = c['qo'].cuda() if new else None
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = paged_attention(*d, qo_indptr=qo, return_lse=True)
+    g.replay(); torch.cuda.synchronize()
+    compare(*got, exact(c))
+print('captured')
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
