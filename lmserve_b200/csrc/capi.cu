@@ -818,7 +818,7 @@ int64_t lms_attention_workspace_bytes(const lms_attention_args* args) {
   if (empty) return 0;
   DeviceState* ds = nullptr;
   if (int rc = device_state(&ds)) return rc;
-  return attention_workspace_bytes(p, ds->sms);
+  return attention_workspace_bytes(p, attention_plan(p, ds->sms));
 }
 
 int lms_paged_attention(const lms_attention_args* args, void* stream) {
@@ -828,7 +828,8 @@ int lms_paged_attention(const lms_attention_args* args, void* stream) {
   if (empty) return LMS_OK;
   DeviceState* ds = nullptr;
   if (int rc = device_state(&ds)) return rc;
-  const int64_t need = attention_workspace_bytes(p, ds->sms);
+  const AttentionPlan plan = attention_plan(p, ds->sms);
+  const int64_t need = attention_workspace_bytes(p, plan);
   if (need > 0) {
     if (!args->workspace) return LMS_ERR_NULL;
     if (((uintptr_t)args->workspace & 255u) != 0) return LMS_ERR_ALIGN;
@@ -838,7 +839,7 @@ int lms_paged_attention(const lms_attention_args* args, void* stream) {
   p.err = ds->err.load(std::memory_order_relaxed);
   p.checks = g_checks.load(std::memory_order_relaxed);
   int launches = 0;
-  LMS_CUDA(launch_attention(p, ds->sms, tuned(LMS_TUNE_WRITE_PDL, 1) == 1, &launches, (cudaStream_t)stream));
+  LMS_CUDA(launch_attention(p, plan, ds->sms, tuned(LMS_TUNE_WRITE_PDL, 1) == 1, &launches, (cudaStream_t)stream));
   g_launches.fetch_add(launches, std::memory_order_relaxed);
   return LMS_OK;
 }

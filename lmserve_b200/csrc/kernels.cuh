@@ -188,8 +188,20 @@ struct AttentionParams {
   int checks;
 };
 
-long long attention_workspace_bytes(const AttentionParams& p, int sms);
-cudaError_t launch_attention(const AttentionParams& p, int sms, bool pdl, int* launches, cudaStream_t stream);
+// What a call launches, from its counts alone.
+struct AttentionPlan {
+  bool rows;                 // the kernel for any head dim does it all
+  bool runs;                 // own keys by the decode kernel
+  int n_ranges, hb_shift, units_per_page;
+  int shared_splits, own_splits;  // key splits of the tile kernel: prefix, own keys (0 = not launched)
+  bool join;
+  long long slots;           // of partials, num_heads rows each
+};
+
+AttentionPlan attention_plan(const AttentionParams& p, int sms);
+long long attention_workspace_bytes(const AttentionParams& p, const AttentionPlan& plan);
+cudaError_t launch_attention(const AttentionParams& p, const AttentionPlan& plan, int sms, bool pdl,
+                             int* launches, cudaStream_t stream);
 
 // ------------------------------------------------------------ per-step index preparation
 struct StepIndexParams {

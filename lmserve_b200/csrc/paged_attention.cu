@@ -248,12 +248,11 @@ struct DecodeParams {
   int box;             // keys of a TMA box
   long long slot0;     // first slot of the runs
   bool join_all;       // whole requests too go to a slot (behind the runs' own): the prefix is joined
-  bool beside;         // runs beside the kernel before it, see wait_before
 };
 
 // Programmatic launches.  A kernel normally waits for the one before it (and lets the one behind it
-// get ready).  The kernel of the own keys needs nothing that the kernel of the shared prefix in
-// front of it writes, only what that one has itself waited for before it let this one start: it
+// get ready).  Of the two kernels of a shared prefix and of the own keys, the second needs nothing
+// that the first writes, only what that one has itself waited for before it let this one start: it
 // runs beside it, on the SMs that are free, and waits behind its work instead, so that what follows
 // (the join) still finds both done.
 __device__ __forceinline__ void wait_before(bool beside) {
@@ -324,11 +323,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
   if (lane < 2) pieces[warp * 2 + lane] = Piece{-1, 0};
   if (TMA) mbar_fence_init();
   __syncwarp();
-  wait_before(p.beside);
-  if (kvh >= a.num_kv_heads) {  // all KS warps of such a head slot leave together
-    wait_behind(p.beside);
-    return;
-  }
+  wait_before(false);
+  if (kvh >= a.num_kv_heads) return;  // all KS warps of such a head slot leave together
 
   // This CTA's run of units, [u_begin, u_end) of the page axis, this warp's part of it, and the
   // request of its first unit: the last b with indptr[b] <= its page, 32 probes a round.
@@ -345,10 +341,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
     const unsigned chunk = (units + p.n_ranges - 1) / p.n_ranges;
     u_begin = chunk * blockIdx.x;
     u_end = min(u_begin + chunk, units);
-    if (u_begin >= u_end) {
-      wait_behind(p.beside);
-      return;
-    }
+    if (u_begin >= u_end) return;
     const unsigned part = (u_end - u_begin + KS - 1) / KS;
     w_begin = min(u_begin + part * ks, u_end);
     w_end = min(w_begin + part, u_end);
@@ -766,7 +759,6 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
   // is in flight when the CTA leaves.
   if (TMA && dead)
     for (int i = max(0, it - NST); i < it; ++i) mbar_wait_bounded(&full[i % NST], (i / NST) & 1);
-  wait_behind(p.beside);
 }
 
 // ---------------------------------------------------------------- tiles of rows
@@ -1611,29 +1603,24 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const J
 }
 
 // ---------------------------------------------------------------- launch rules
-// What a call launches, from its counts alone.
-struct Plan {
-  bool rows;                 // the kernel for any head dim does it all
-  bool runs;                 // own keys by the decode kernel
-  int n_ranges, hb_shift, units_per_page;
-  int shared_splits, own_splits;  // key splits of the tile kernel: prefix, own keys (0 = not launched)
-  bool join;
-  long long slots;           // of partials, num_heads rows each
-};
+// Pairs of row tiles of a key head: every sequence has one at least.
+long long row_tiles(long long tokens, long long seqs, const AttentionParams& p) {
+  const long long tiles = (tokens * (p.num_heads / p.num_kv_heads) + 2 * kRows - 1) / (2 * kRows);
+  return tiles < seqs ? seqs : tiles;
+}
 
-// Splits of the keys so that the row tiles fill the GPU, a tile of keys each at least.
+// Splits of the keys so that the row tiles fill the GPU, a tile of keys each at least.  (Twice or three
+// times the pieces: 256 requests behind 8192 keys 108 and 114 us instead of 100.)
 int splits_of(long long tokens, long long seqs, long long pages, const AttentionParams& p, int sms) {
-  const int G = p.num_heads / p.num_kv_heads;
-  long long tiles = (tokens * G + 2 * kRows - 1) / (2 * kRows);
-  if (tiles < seqs) tiles = seqs;
   const long long keys = pages * p.block_size / (seqs > 0 ? seqs : 1);
-  long long n = sms / (tiles * p.num_kv_heads);
+  const long long tiles = row_tiles(tokens, seqs, p);
+  long long n = sms / ((tiles > 0 ? tiles : 1) * p.num_kv_heads);
   if (n > keys / kKeys) n = keys / kKeys;
   return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 
-Plan plan_of(const AttentionParams& p, int sms) {
-  Plan r{};
+AttentionPlan plan_of(const AttentionParams& p, int sms) {
+  AttentionPlan r{};
   const int G = p.num_heads / p.num_kv_heads;
   const bool shared = p.prefix.indptr != nullptr;
   r.units_per_page = (p.block_size + kTile - 1) / kTile;
@@ -1650,7 +1637,40 @@ Plan plan_of(const AttentionParams& p, int sms) {
     auto blocks = [&](int s) { return (p.num_kv_heads + (1 << s) - 1) >> s; };
     while (shift > 0 && units * blocks(shift) < 16ll * sms) --shift;
     r.hb_shift = shift;
-    r.n_ranges = sms / blocks(shift);
+    int run_sms = sms;
+    if (shared) {
+      // Beside the tiles of a prefix the runs take some of the SMs, and the prefix's pieces go over the
+      // others in whole rounds: the pair of shares and splits that ends first, by what either takes on
+      // an SM - 0.19 us a 16-key unit of a head of 128 (43 GB/s), 1.7 us a key tile and 8 us a piece -
+      // and what the join reads.  (256 requests behind 8192 keys: 104 us one behind the other, 100 with
+      // half the SMs each, 114 where the pieces leave a third round; 8 groups: 58 to 48 us.)
+      const double own = (double)units * p.num_kv_heads * p.head_dim * (0.19 / 128);
+      const double tiles = (double)row_tiles(p.num_tokens, p.num_groups, p) * p.num_kv_heads;
+      const long long keys = p.prefix.num_indices * p.block_size / (p.num_groups > 0 ? p.num_groups : 1);
+      const double key_tiles = (double)((keys + kKeys - 1) / kKeys);
+      const double part = (double)p.num_tokens * p.num_heads * p.head_dim * 8 / 6e6;
+      // several prefixes: the counts give their mean, the longest may be twice that
+      const double longest = p.num_groups > 1 ? 1 : 0;
+      auto piece = [&](double splits) { return key_tiles / splits * 1.7 + 8; };
+      auto tiles_end = [&](double rounds, double splits) { return rounds * piece(splits) + longest * key_tiles / splits * 1.7; };
+      const double all = r.shared_splits;  // one behind the other, each on all SMs
+      double best = own / sms + 6 + tiles_end((double)(((long long)(tiles * all) + sms - 1) / sms), all) + all * part;
+      const int most = key_tiles < 12 ? (int)key_tiles : 12;
+      for (int splits = 1; splits <= most; ++splits)
+        for (int rounds = 1; rounds <= 3; ++rounds) {
+          const long long left = ((long long)tiles * splits + rounds - 1) / rounds;
+          const long long mine = sms - left;
+          if (mine < 2 * sms / 5) continue;
+          const double ends = own / mine + 6, t = tiles_end(rounds, splits);
+          const double total = (t > ends ? t : ends) + splits * part;
+          if (total < best) {
+            best = total;
+            run_sms = (int)mine;
+            r.shared_splits = splits;
+          }
+        }
+    }
+    r.n_ranges = run_sms / blocks(shift);
     if (r.n_ranges < 1) r.n_ranges = 1;
     r.slots = 2ll * r.n_ranges + (shared ? p.num_requests : 0);
     r.join = true;
@@ -1664,7 +1684,7 @@ Plan plan_of(const AttentionParams& p, int sms) {
 
 long long align256(long long x) { return (x + 255) & ~255ll; }
 
-Partials partials_at(const AttentionParams& p, const Plan& plan) {
+Partials partials_at(const AttentionParams& p, const AttentionPlan& plan) {
   Partials r;
   r.lse = reinterpret_cast<float*>(p.workspace);
   r.out = reinterpret_cast<float*>(p.workspace + align256(plan.slots * p.num_heads * 4));
@@ -1729,7 +1749,7 @@ cudaError_t allow_smem(K kernel, int most, std::atomic<unsigned long long>* aske
 }
 
 template <bool BF16, int D, int NT, int NST>
-cudaError_t launch_decode(const AttentionParams& p, const Plan& plan, bool pdl, cudaStream_t stream) {
+cudaError_t launch_decode(const AttentionParams& p, const AttentionPlan& plan, bool pdl, cudaStream_t stream) {
   DecodeParams d{};
   d.a = p;
   d.part = partials_at(p, plan);
@@ -1737,7 +1757,7 @@ cudaError_t launch_decode(const AttentionParams& p, const Plan& plan, bool pdl, 
   d.hb_shift = plan.hb_shift;
   d.units_per_page = plan.units_per_page;
   d.slot0 = (long long)(plan.shared_splits + plan.own_splits) * p.num_tokens;
-  d.join_all = d.beside = plan.shared_splits > 0;
+  d.join_all = plan.shared_splits > 0;
   const int G = p.num_heads / p.num_kv_heads, HB = 1 << plan.hb_shift;
   d.box = p.block_size % kTile == 0 ? kTile : p.block_size == 8 ? 8 : 0;
   const bool tma = d.box > 0 && encode_plane(p, p.kcache, d.box, &d.kmap) && encode_plane(p, p.vcache, d.box, &d.vmap);
@@ -1751,7 +1771,7 @@ cudaError_t launch_decode(const AttentionParams& p, const Plan& plan, bool pdl, 
 }
 
 template <bool BF16, int D>
-cudaError_t launch_tile(const AttentionParams& p, const Plan& plan, bool shared, bool pdl, cudaStream_t stream) {
+cudaError_t launch_tile(const AttentionParams& p, const AttentionPlan& plan, bool shared, bool beside, bool pdl, cudaStream_t stream) {
   TileParams t{};
   t.a = p;
   t.list = shared ? p.prefix : p.own;
@@ -1765,7 +1785,7 @@ cudaError_t launch_tile(const AttentionParams& p, const Plan& plan, bool shared,
   t.n_slots = (int)slots;
   t.slot0 = plan.join ? (shared ? 0 : plan.shared_splits) : -1;
   t.causal = !shared && p.causal;
-  t.beside = !shared && plan.shared_splits > 0;
+  t.beside = beside;
   const int bs = p.block_size;
   if (bs % kKeys == 0) t.box = kKeys;
   else if (bs >= 8 && bs < kKeys && kKeys % bs == 0) t.box = bs;
@@ -1782,7 +1802,7 @@ cudaError_t launch_tile(const AttentionParams& p, const Plan& plan, bool shared,
 }
 
 template <bool BF16, int D>
-cudaError_t launch_join(const AttentionParams& p, const Plan& plan, int sms, bool pdl, cudaStream_t stream) {
+cudaError_t launch_join(const AttentionParams& p, const AttentionPlan& plan, int sms, bool pdl, cudaStream_t stream) {
   JoinParams j{};
   j.a = p;
   j.part = partials_at(p, plan);
@@ -1808,20 +1828,29 @@ cudaError_t launch_rows(const AttentionParams& p, bool pdl, cudaStream_t stream)
 }
 
 template <bool BF16, int D>
-cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, int sms, bool pdl, int* launches, cudaStream_t stream) {
+cudaError_t launch_matrix(const AttentionParams& p, const AttentionPlan& plan, int sms, bool pdl, int* launches, cudaStream_t stream) {
+  const bool shared = plan.shared_splits > 0;
   cudaError_t e = cudaSuccess;
-  if (plan.shared_splits > 0) {
-    e = launch_tile<BF16, D>(p, plan, true, pdl, stream);
-    *launches += e == cudaSuccess;
-  }
-  if (e == cudaSuccess && plan.runs) {
+  if (plan.runs) {
+    // the runs take their share of the SMs (plan_of) and leave the others to the prefix
     const bool few = p.num_heads / p.num_kv_heads <= 8;
     constexpr int kDeep = D == 64 ? 6 : 3;
     e = few ? launch_decode<BF16, D, 1, kDeep>(p, plan, pdl, stream) : launch_decode<BF16, D, 2, D == 64 ? 5 : 2>(p, plan, pdl, stream);
     *launches += e == cudaSuccess;
-  } else if (e == cudaSuccess) {
-    e = launch_tile<BF16, D>(p, plan, false, pdl, stream);
-    *launches += e == cudaSuccess;
+    if (e == cudaSuccess && shared) {
+      e = launch_tile<BF16, D>(p, plan, true, true, pdl, stream);
+      *launches += e == cudaSuccess;
+    }
+  } else {
+    // few long pieces first, the short ones of the own keys on the SMs that they leave
+    if (shared) {
+      e = launch_tile<BF16, D>(p, plan, true, false, pdl, stream);
+      *launches += e == cudaSuccess;
+    }
+    if (e == cudaSuccess) {
+      e = launch_tile<BF16, D>(p, plan, false, shared, pdl, stream);
+      *launches += e == cudaSuccess;
+    }
   }
   if (e == cudaSuccess && plan.join) {
     e = launch_join<BF16, D>(p, plan, sms, pdl, stream);
@@ -1831,7 +1860,7 @@ cudaError_t launch_matrix(const AttentionParams& p, const Plan& plan, int sms, b
 }
 
 template <bool BF16>
-cudaError_t launch_typed(const AttentionParams& p, const Plan& plan, int sms, bool pdl, int* launches, cudaStream_t stream) {
+cudaError_t launch_typed(const AttentionParams& p, const AttentionPlan& plan, int sms, bool pdl, int* launches, cudaStream_t stream) {
   if (plan.rows) {
     *launches = 1;
     return launch_rows<BF16>(p, pdl, stream);
@@ -1842,14 +1871,14 @@ cudaError_t launch_typed(const AttentionParams& p, const Plan& plan, int sms, bo
 
 }  // namespace
 
-long long attention_workspace_bytes(const AttentionParams& p, int sms) {
-  const Plan plan = plan_of(p, sms);
+AttentionPlan attention_plan(const AttentionParams& p, int sms) { return plan_of(p, sms); }
+
+long long attention_workspace_bytes(const AttentionParams& p, const AttentionPlan& plan) {
   if (plan.slots == 0) return 0;
   return align256(plan.slots * p.num_heads * 4) + align256(plan.slots * p.num_heads * p.head_dim * 4);
 }
 
-cudaError_t launch_attention(const AttentionParams& p, int sms, bool pdl, int* launches, cudaStream_t stream) {
-  const Plan plan = plan_of(p, sms);
+cudaError_t launch_attention(const AttentionParams& p, const AttentionPlan& plan, int sms, bool pdl, int* launches, cudaStream_t stream) {
   *launches = 0;
   return p.is_bf16 ? launch_typed<true>(p, plan, sms, pdl, launches, stream)
                    : launch_typed<false>(p, plan, sms, pdl, launches, stream);
