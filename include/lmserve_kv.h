@@ -355,7 +355,9 @@ int lms_qk_norm_rope_and_cache(const lms_qk_norm_args* args, void* stream);
  * `workspace`: lms_attention_workspace_bytes(args) bytes of device memory, 256-byte aligned, that
  * no other call in flight uses; its contents need not be kept or cleared.  The size depends on
  * the counts in `args` alone, not on the arrays' contents.
- * dtype 0 = fp16, 1 = bf16; head_dim a multiple of 8 up to 256.
+ * dtype 0 = fp16, 1 = bf16; head_dim a multiple of 8 up to 256 (64 and 128 run on the tensor cores,
+ * the others on the CUDA cores).  (num_*_indices + 1) * (block_size + 16) and num_tokens * num_heads /
+ * num_kv_heads must stay below 2^31.
  */
 typedef struct lms_attention_args {
   const void* query;

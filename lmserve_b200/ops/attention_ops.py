@@ -92,6 +92,8 @@ def _refuse(query, paged_kv_cache, lists, qo_indptr, group_indptr, out):
 
 
 def _check_index(name: str, t: torch.Tensor, dev: torch.device) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if t.dtype != _I32:
         raise TypeError(f"{name} must be int32 (got {t.dtype})")
     if t.device != dev or t.dim() != 1 or not t.is_contiguous():
@@ -99,6 +101,8 @@ def _check_index(name: str, t: torch.Tensor, dev: torch.device) -> None:
 
 
 def _attention(query, paged_kv_cache: Cache, own, prefix, group_indptr, qo_indptr, scale, causal, return_lse, out):
+    if not isinstance(query, torch.Tensor):
+        raise TypeError(f"query must be a torch.Tensor, got {type(query).__name__}")
     idx = query.get_device()
     if idx >= 0 and idx != _current_device():
         with torch.cuda.device(idx):
@@ -150,7 +154,8 @@ def paged_attention(query: torch.Tensor, paged_kv_cache: Cache, kv_indptr: torch
     ``qo_indptr[0]:qo_indptr[-1]`` (a padded batch) are not written: pass ``out`` (same shape and
     dtype, sharing no memory with the inputs) to say what they hold.
 
-    Head dims up to 256 that are multiples of 8.
+    Head dims up to 256 that are multiples of 8; 64 and 128 run on the tensor cores, the others on the
+    CUDA cores, which is slow for prompts.  Forward only: nothing is recorded for a gradient.
     """
     return _attention(query, paged_kv_cache, (kv_indptr, kv_indices, kv_last_page_len), (None, None, None), None,
                       qo_indptr, scale, causal, return_lse, out)

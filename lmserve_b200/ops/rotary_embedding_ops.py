@@ -159,6 +159,11 @@ def rotary_pos_emb_and_cache(query: torch.Tensor, key: torch.Tensor, value: torc
 _qk_norm_entry: Optional[int] = None
 
 
+def _require_tensor(name, t):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+
+
 def _refuse_qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cache, head_dim, kv_cache, slots):
     """Names what is wrong with the arguments of a head norm + rotary call."""
     for n, t in (("query_weight", query_weight), ("key_weight", key_weight)):
@@ -196,6 +201,7 @@ def _refuse_qk_norm(query, key, value, query_weight, key_weight, positions, cos_
 
 def _qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps,
              kv_cache, slot_mapping, return_key):
+    _require_tensor("query", query)
     idx = query.get_device()
     if idx >= 0 and idx != _current_device():
         with torch.cuda.device(idx):

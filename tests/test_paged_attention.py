@@ -427,6 +427,10 @@ def test_refusals_gpu():
         f(q=c["q"])
     with pytest.raises(ValueError, match="cache's device"):
         f(own=list(c["own"]))
+    with pytest.raises(TypeError, match="torch.Tensor"):
+        f(own=[own[0], None, own[2]])
+    with pytest.raises(TypeError, match="torch.Tensor"):
+        f(q=None)
     with pytest.raises(TypeError, match="int32"):
         f(own=[own[0].long(), *own[1:]])
     with pytest.raises(TypeError, match="one dtype"):
