@@ -225,16 +225,16 @@ struct Partials {
 // earlier run, else 2x + 1) for the join kernel.
 //
 // Inside a CTA a warp works alone: head hs = w % HB of the block, the ks-th of KS = 8 / HB equal parts
-// of the run, its own ring of stages filled by TMA (a box a page, 128-byte swizzled) or, for page
-// sizes a 16-key box does not fit, by cp.async rows; no barrier in the loop.  Both
+// of the run, its own ring of stages filled by TMA (a box a page, 128-byte swizzled) or, for many
+// bytes and for page sizes a 16-key box does not fit, by cp.async rows; no barrier in the loop.  Both
 // products are taken transposed, S^T = K Q^T and O^T += V^T P^T (m16n8k16), so that the 16-wide
 // side is full of keys or head elements and the 8-wide side holds the G rows: half the products and
 // registers of the other way round for G <= 8.  S^T turns into the second product's operand with
 // movmatrix.  Measured (HBM copy rate 6.55 TB/s): 256 requests of up to 4000 keys, 8 key heads of 128,
-// 2.1 GB in 329 us, 6.4 TB/s; 512 requests of up to 1500 keys on one key head, 225 MB in 50 us, 4.5 TB/s:
-// the first tiles are there after 4 to 5 us, the SMs' shares of the bandwidth differ by 15 %, and the
-// slowest of the equal runs decides.  What the borders between the KS parts cut is joined through shared memory at the end
-// (one barrier a CTA; a barrier a request, with the tiles dealt out in turn, cost 2 to 4 us each).
+// 2.1 GB in 308 to 314 us (324 among other work), 6.5 to 6.7 TB/s; 512 requests of up to 1500 keys on one
+// key head, 225 MB in 50 us, 4.5 TB/s: the first tiles are there after 4 to 5 us, the SMs' shares of the bandwidth differ by 15 %, and the
+// slowest of the equal runs decides.  What the borders between the KS parts cut is joined through shared
+// memory at the end (one barrier a CTA; a barrier a request, with the tiles dealt out in turn, cost 2 to 4 us each).
 constexpr int kDecodeWarps = 8;
 constexpr int kTile = 16;  // keys
 
@@ -1759,7 +1759,15 @@ cudaError_t launch_decode(const AttentionParams& p, const AttentionPlan& plan, b
   d.slot0 = (long long)(plan.shared_splits + plan.own_splits) * p.num_tokens;
   d.join_all = plan.shared_splits > 0;
   const int G = p.num_heads / p.num_kv_heads, HB = 1 << plan.hb_shift;
-  d.box = p.block_size % kTile == 0 ? kTile : p.block_size == 8 ? 8 : 0;
+  // Below 512 MB of pages the boxes are as fast as rows or faster, since they cost fewer instructions
+  // (256 requests of up to 512 keys, 8 key heads of 128, beside an 8192-key prefix: 91 us, by rows 92; 300 of
+  // up to 200 keys, 37.6 and 39.0; 8 prefixes of up to 4000, 49.1 and 50.4).  Above it HBM alone counts, and
+  // the rows' 16-byte requests keep it busier (256 requests of up to 4000 keys 330 us, by rows 314; with
+  // pages of 32 keys 334 and 310; 64 of up to 16000, 4 heads of 64, 138 and 135).  At 524 MB they are equal.
+  // Among other kernels that leave the L2 cache full of written lines both take 324 us for the first of these.
+  const double bytes = 4.0 * p.own.num_indices * p.block_size * p.num_kv_heads * D;
+  const bool rows = bytes > 512.0 * (1 << 20);
+  d.box = rows ? 0 : p.block_size % kTile == 0 ? kTile : p.block_size == 8 ? 8 : 0;
   const bool tma = d.box > 0 && encode_plane(p, p.kcache, d.box, &d.kmap) && encode_plane(p, p.vcache, d.box, &d.vmap);
   auto kernel = tma ? attention_decode_kernel<BF16, D, NT, NST, true> : attention_decode_kernel<BF16, D, NT, NST, false>;
   const int smem = DecodeSmem<D, NST>::bytes(G, HB);

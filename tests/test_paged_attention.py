@@ -568,6 +568,28 @@ def test_thousands_of_requests():
 
 
 @gpu
+@pytest.mark.parametrize("D,dtype", [(128, BF), (64, HF)])
+@pytest.mark.parametrize("prefix", [None, [1000]])
+def test_many_bytes_of_keys(prefix, D, dtype):
+    """Above the size where the decode kernel fetches rows in place of boxes: 0.6 GB of table, on few pages."""
+    once, times = [4000, 17, 0, 4099, 1, 900], 30 * 256 // D
+    c = case(once, HQ=16, H=8, D=D, dtype=dtype, prefix=prefix)
+    indptr, indices, last = c["own"]
+    ends = torch.cat([indptr[1:] + i * int(indptr[-1]) for i in range(times)])
+    c["own"] = (torch.cat([indptr[:1], ends]).int(), indices.repeat(times), last.repeat(times))
+    assert len(c["own"][1]) * 16 * 8 * D * 4 > 2**29
+    g = torch.Generator().manual_seed(2)
+    c["q"] = (2 * torch.randn(len(once) * times, 16, D, generator=g)).to(dtype)
+    out, lse = call(c, return_lse=True)
+    some = list(range(len(once) * 7, len(once) * 9)) + list(range(len(once) * (times - 1), len(once) * times))
+    start = c["own"][0].tolist()
+    lists = [c["own"][1][start[b]:start[b + 1]].tolist() for b in some]
+    picked = dict(c, q=c["q"][some], own=(torch.tensor([0, *torch.tensor([len(x) for x in lists]).cumsum(0)], dtype=torch.int32),
+                                          torch.tensor(sum(lists, []), dtype=torch.int32), c["own"][2][some]))
+    compare(out[some], lse[some], exact(picked))
+
+
+@gpu
 def test_the_first_call_may_be_captured():
     """In a fresh process: per-device set-up, then a capture with no call before it."""
     import subprocess
