@@ -735,7 +735,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
           const float* src = i & 1 ? reinterpret_cast<const float*>(smem + w * NST * S::kStage) : heads + w * G * D;
           const float4 v = *reinterpret_cast<const float4*>(src + r * D + d);
           const float pm = stat[r], pl = stat[G + r];
-          if (pm == -INFINITY) continue;  // a piece without a key
+          // A piece without a key has the sum 0.  Its maximum says less: NaN scores do not move it, and
+          // their sum, NaN, has to reach the row.
+          if (pl == 0.f) continue;
           const float top = fmaxf(mm, pm), keep = exp2_fast(mm - top), f = exp2_fast(pm - top);
           mm = top;
           ll = fmaf(ll, keep, f * pl);
