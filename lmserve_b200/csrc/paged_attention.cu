@@ -76,8 +76,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 
 // One warp, one row: a lane owns the element pairs lane, lane + 32, ... of the head, up to PAIRS of
 // them.  Scores in base 2.  Keys that are not walked are not touched.
-template <bool BF16, int PAIRS>
+template <bool BF16>
 struct RowWalk {
+  static constexpr int PAIRS = 4;
   float2 q[PAIRS], acc[PAIRS];
   float m = -INFINITY, l = 0.f;
 
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(128) attention_rows_kernel(const AttentionPara
     i = t - p.qo_indptr[b];
   }
   const int kvh = h / (p.num_heads / p.num_kv_heads);
-  RowWalk<BF16, 4> w(p.q + (long long)t * p.q_tok + (long long)h * p.head_dim * 2, p.head_dim, lane);
+  RowWalk<BF16> w(p.q + (long long)t * p.q_tok + (long long)h * p.head_dim * 2, p.head_dim, lane);
   if (p.prefix.indptr != nullptr) {
     const int g = p.group_indptr != nullptr ? last_not_above(p.group_indptr, p.num_groups + 1, b) : 0;
     if (g >= 0 && g < p.num_groups)
@@ -821,8 +822,9 @@ struct TileSmem {
 
 struct TileBars {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-  uint64_t wfull[2], wempty[2], qfull[2], sfull[2], pfull[2][2], ofull[2], want, grant, done;
+  uint64_t wfull[2], wempty[2], qfull[2], sfull[2], pfull[2][2], ofull[2], vraw, want, grant, done;
   uint32_t tmem;
+  int cleaned[4];  // of the it-th piece, at it % 4: 1 + the first tile of V that lost an element to clean_tile, or 0
 };
 
 // Two row tiles of one key head against a run of key tiles.
@@ -832,6 +834,12 @@ struct TileWork {
   int len, first_page;    // keys of the sequence, place of its first page in the list
   int tile0, n_kv;        // key tiles
   int kvh, split;
+
+  // The first key that a row of the pair does not read although another may: causal rows read up to
+  // their own token, and the first row's is the earliest.
+  __device__ __forceinline__ int first_hidden(bool causal, int G) const {
+    return causal ? min(len, max(0, len - n_new + row0 / G + 1)) : len;
+  }
 };
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -994,6 +1002,38 @@ __device__ __forceinline__ void load_tile(const TileParams& p, const CUtensorMap
   if (lane == 0) mbar_arrive(full);
 }
 
+// Sets what is infinite or NaN in a stage of V to 0; true if there was anything.  One warp.
+template <bool BF16, int D>
+__device__ __forceinline__ bool clean_tile(uint32_t tile, int lane) {
+  // an exponent of ones carries into bit 15 of its half word
+  constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
+  constexpr int kBatch = 4;
+  auto load = [&](int c, uint32_t* v) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(tile + c * 16) : "memory");
+  };
+  uint32_t found = 0;
+#pragma unroll 1
+  for (int c = lane; c < kKeys * D / 8; c += 32 * kBatch) {
+    uint32_t v[kBatch][4];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) load(c + 32 * i, v[i]);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) found |= (v[i][w] & kExp) + kOne;
+  }
+  if (!__any_sync(0xffffffffu, (found & 0x80008000u) != 0)) return false;
+#pragma unroll 1
+  for (int c = lane; c < kKeys * D / 8; c += 32) {
+    uint32_t v[4];
+    load(c, v);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v[w] &= ~(((((v[w] & kExp) + kOne) & 0x80008000u) >> 15) * 0xffffu);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + c * 16), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+  }
+  return true;
+}
+
 template <bool BF16, int D>
 __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const __grid_constant__ TileParams p) {
   using S = TileSmem<D>;
@@ -1023,6 +1063,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
       mbar_init(&bars.pfull[i][1], 4);
       mbar_init(&bars.ofull[i], 1);
     }
+    mbar_init(&bars.vraw, 1);
     mbar_init(&bars.want, 1);
     mbar_init(&bars.grant, 1);
     mbar_init(&bars.done, 1);
@@ -1212,7 +1253,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays
         // O leaves through the shared memory of the warp's own Q rows, which nothing reads any more: a
         // thread has a row, a store instruction should have whole 128-byte lines.
-        float finite = 0.f;
         const unsigned have = __ballot_sync(0xffffffffu, has_row);
         const uint32_t stage = sm_q + i * kRows * D * 2 + (warp & 3) * 32 * 128;
         auto emit = [&](auto part) {
@@ -1228,13 +1268,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
 #pragma unroll
             for (int c = 0; c < kCols; c += 32) tc_ld32(o + c, t_o + pass * kCols + c);
             tc_wait_ld();
-            float odd[4] = {0.f, 0.f, 0.f, 0.f};  // NaN where an element is not finite
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-              odd[c & 3] = fmaf(__uint_as_float(o[c]), 0.f, odd[c & 3]);
-              o[c] = __float_as_uint(__uint_as_float(o[c]) * inv);
-            }
-            finite += (odd[0] + odd[1]) + (odd[2] + odd[3]);
+            for (int c = 0; c < kCols; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * inv);
             constexpr int kPer = PART ? 4 : 8;  // values of a 16-byte chunk
 #pragma unroll
             for (int e = 0; e < kCols; e += kPer) {
@@ -1274,28 +1309,41 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           if (p.slot0 >= 0) p.part.lse[part_row] = lse2;
           else if (a.lse != nullptr) a.lse[out_row] = lse2 * kLn2;
         }
-        // A key masked for this row but not for the whole tile took part in PV with weight 0, and
-        // 0 * infinity is NaN: a causal row that is not finite is done again by itself.
-        __syncwarp();
-        unsigned again = __ballot_sync(0xffffffffu, p.causal && has_row && finite != 0.f);
-        while (again != 0) {
-          const int who = __ffs(again) - 1;
-          again &= again - 1;
-          const int w_tok = __shfl_sync(0xffffffffu, tok, who), w_g = __shfl_sync(0xffffffffu, g, who);
-          const int w_end = min(__shfl_sync(0xffffffffu, limit, who), (k.tile0 + k.n_kv) * kKeys);
-          const long long w_part = __shfl_sync(0xffffffffu, part_row, who), w_out = __shfl_sync(0xffffffffu, out_row, who);
-          const long long head = (long long)(k.kvh * G + w_g) * D * 2;
-          RowWalk<BF16, D / 64> walk(a.q + (long long)(k.t_begin + w_tok) * a.q_tok + head, D, lane);
-          walk.walk(a, p.list, k.first_page, k.kvh, k.tile0 * kKeys, w_end, lane);
-          if (p.slot0 < 0) {
-            walk.store(a.out + (long long)(k.t_begin + w_tok) * a.o_tok + head, D, lane);
-            if (a.lse != nullptr && lane == 0) a.lse[w_out] = walk.lse2() * kLn2;
-          } else {
+        // What clean_tile took out of V reaches the rows that read its key: infinity or NaN, whatever
+        // the weight.  Limits rise from row to row, so one walk over the tiles with keys that are hidden from
+        // some row (those of 256 / G tokens, and the tile they begin in) serves the warp.
+        if (const int from = bars.cleaned[it & 3]) {
+          __syncwarp();
+          float2 odd[D / 64] = {};
+          int key = (from - 1) * kKeys;
+          for (int who = 0; who < 32 && (have >> who & 1); ++who) {
+            const int end = min(__shfl_sync(0xffffffffu, limit, who), (k.tile0 + k.n_kv) * kKeys);
+            const long long w_part = __shfl_sync(0xffffffffu, part_row, who);
+            const int w_tok = __shfl_sync(0xffffffffu, tok, who), w_g = __shfl_sync(0xffffffffu, g, who);
+            for (; key < end; ++key) {
+              const long long off = key_offset(a, p.list, k.first_page, key);
+              if (off < 0) continue;
+              const uint32_t* v = reinterpret_cast<const uint32_t*>(a.vcache + off + (long long)k.kvh * D * 2);
 #pragma unroll
-            for (int e = 0; e < D / 64; ++e)
-              reinterpret_cast<float2*>(p.part.out + w_part * D)[lane + 32 * e] =
-                  make_float2(walk.acc[e].x * walk.inverse(), walk.acc[e].y * walk.inverse());
-            if (lane == 0) p.part.lse[w_part] = walk.lse2();
+              for (int e = 0; e < D / 64; ++e) {
+                const float2 f = up2<BF16>(v[lane + 32 * e]);
+                if (!(fabsf(f.x) < INFINITY)) odd[e].x += f.x;
+                if (!(fabsf(f.y) < INFINITY)) odd[e].y += f.y;
+              }
+            }
+            if (__shfl_sync(0xffffffffu, l, who) == 0.f) continue;  // it reads no key
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e) {
+              if (odd[e].x == 0.f && odd[e].y == 0.f) continue;
+              if (p.slot0 >= 0) {
+                float2* const o = reinterpret_cast<float2*>(p.part.out + w_part * D) + lane + 32 * e;
+                *o = make_float2(o->x + odd[e].x, o->y + odd[e].y);
+              } else {
+                uint32_t* const o = reinterpret_cast<uint32_t*>(a.out + (long long)(k.t_begin + w_tok) * a.o_tok + (long long)(k.kvh * G + w_g) * D * 2) + lane + 32 * e;
+                const float2 f = up2<BF16>(*o);
+                *o = down2<BF16>(f.x + odd[e].x, f.y + odd[e].y);
+              }
+            }
           }
         }
         tc_fence_before();
@@ -1310,19 +1358,36 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     uint64_t* full = is_k ? bars.kfull : bars.vfull;
     uint64_t* empty = is_k ? bars.kempty : bars.vempty;
     int n = 0;  // tiles loaded so far
+    int held = 0;  // of them, those looked through
     bool ok = true;
     for (int it = 0; ok; ++it) {
       const TileWork k = next_work(it);
       if (k.rows == 0) break;
+      // A key that is hidden from a row takes part in its PV with weight 0, and 0 * infinity is NaN: the
+      // tiles of V with such keys are looked through before the MMAs get them.
+      const int hidden = is_k ? k.len : k.first_hidden(p.causal, G);
+      if (!is_k && lane == 0) bars.cleaned[it & 3] = 0;  // whoever reads that of piece it - 4 is past it
       for (int j = 0; j < k.n_kv; ++j, ++n) {
         const int s = n % ST, use = n / ST;
         if (use > 0 && !(ok = wait(&empty[s], (use - 1) & 1))) break;
+        const bool hold = hidden < k.len && (k.tile0 + j + 1) * kKeys > hidden;
+        const uint32_t dst = (is_k ? sm_k : sm_v) + s * S::kStage;
         load_tile<D>(p, is_k ? &p.kmap : &p.vmap, is_k ? a.kcache : a.vcache, k.kvh, k.first_page, k.len, k.tile0 + j,
-                     (is_k ? sm_k : sm_v) + s * S::kStage, &full[s], lane);
+                     dst, hold ? &bars.vraw : &full[s], lane);
+        if (hold) {
+          if (!(ok = wait(&bars.vraw, held++ & 1))) break;
+          if (clean_tile<BF16, D>(dst, lane)) {
+            fence_proxy_async();
+            if (lane == 0 && bars.cleaned[it & 3] == 0) bars.cleaned[it & 3] = k.tile0 + j + 1;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[s]);
+        }
       }
       if (is_k && lane == 0) mbar_arrive(&bars.want);  // time to look for more
     }
     // no copy may be in flight when the CTA leaves, whatever the others did
+    if (!ok && held > 0) wait(&bars.vraw, (held - 1) & 1);
     for (int d = max(0, n - ST); d < n; ++d) wait(&full[d % ST], (d / ST) & 1);
   } else if (warp == 10) {
     // ------------------------------------------------ MMAs

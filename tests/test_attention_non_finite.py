@@ -47,3 +47,73 @@ def test_nan_keys(lengths, HQ, H, D, dtype, new):
     pages = c["own"][1][c["own"][0][at]:c["own"][0][at + 1]]
     c["cache"][pages[len(pages) // 2].item(), 0, :, H - 1] = math.nan
     same(*call(c, return_lse=True), exact(c))
+
+
+def bounded(c, clean, **kw):
+    """The formula on `c`, with the bounds of the same call without what is infinite or NaN in V."""
+    o, _, l, _ = exact(c, **kw)
+    _, ob, _, lb = exact(clean, **kw)
+    return o, ob, l, lb
+
+
+def with_values(c, at, what):
+    """(a copy of `c` with these values at (request, key, key head, element) of V, `c`)."""
+    bs = c["cache"].shape[2]
+    dirty = dict(c, cache=c["cache"].clone())
+    for (b, key, h, e), x in zip(at, what):
+        page = c["own"][1][c["own"][0][b] + key // bs].item()
+        dirty["cache"][page, 1, key % bs, h, e] = x
+    return dirty, c
+
+
+PROMPTS = [([300], [300]), ([700, 40, 129], [500, 40, 1]), ([600, 2], [257, 2]), ([50, 260], [90, 300])]
+
+
+@gpu
+@pytest.mark.parametrize("prefix", [None, [150]])
+@pytest.mark.parametrize("BS", [16, 12, 128])
+@pytest.mark.parametrize("HQ,H,D,dtype", [(8, 2, 128, BF), (3, 3, 64, HF), (14, 2, 128, HF), (20, 1, 64, BF)])
+@pytest.mark.parametrize("lengths,new", PROMPTS)
+def test_infinite_values_of_prompts(lengths, new, HQ, H, D, dtype, BS, prefix):
+    """Seen by some rows and hidden from others: among the first keys, in the middle, and the last."""
+    n = lengths[0]
+    at = [(0, 0, 0, 3), (0, n // 2, 0, 4), (0, n - 20, 0, 5), (0, n - 1, 0, 3), (0, n - 1, H - 1, D - 1), (0, n // 2, H - 1, 7), (0, n - 9, H - 1, 7)]
+    what = [math.inf, -math.inf, math.nan, -math.inf, math.inf, math.inf, math.inf]
+    dirty, clean = with_values(case(lengths, new, HQ=HQ, H=H, D=D, dtype=dtype, BS=BS, prefix=prefix, spread=0.5), at, what)
+    same(*call(dirty, return_lse=True), bounded(dirty, clean))
+
+
+@gpu
+@pytest.mark.parametrize("what", ["query", "first value", "last value"])
+def test_what_is_not_finite_costs_no_walk_over_the_keys(what):
+    c = case([2048], [2048], HQ=8, H=2)
+    if what == "query":
+        dirty = dict(c, q=c["q"].clone())
+        dirty["q"][:, :, 0] = math.nan
+    else:
+        key = 0 if what == "first value" else 2047
+        dirty, _ = with_values(c, [(0, key, 0, 0), (0, key, 1, 0)], [math.inf, math.inf])
+    from lmserve_b200.ops import paged_attention
+
+    def time(c):
+        args = [t.to("cuda:0") for t in (c["q"], c["cache"], *c["own"])]
+        qo, best = c["qo"].to("cuda:0"), math.inf
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            paged_attention(*args, qo_indptr=qo)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    assert time(dirty) < 8 * time(c)
+
+
+@gpu
+def test_infinite_values_of_the_newest_tokens_of_a_long_request():
+    n = 50_000
+    c = case([9, n, 300], [9, 40, 1], HQ=2, H=1, D=64, spread=0.5)
+    at = [(1, n - 1, 0, 1), (1, n - 30, 0, 2), (1, n - 41, 0, 3), (1, 3, 0, 4)]
+    dirty, clean = with_values(c, at, [math.inf, -math.inf, math.inf, math.inf])
+    same(*call(dirty, return_lse=True), bounded(dirty, clean))
