@@ -208,7 +208,17 @@ __device__ __forceinline__ void tma_load4(uint32_t dst, const CUtensorMap* map, 
       "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
 }
-constexpr float kLazy = 8.f;     // log2 of the factor a running maximum may lag behind
+// Weights of the matrix kernels are 2^(s - m) with m at least kBelow under the largest score so far;
+// m moves when a score passes it by more than kReach.  bf16 has the exponents of fp32: m may lag 8
+// behind.  fp16 has 2^15 for its largest power and 2^-25 for half its smallest step, so it takes weights
+// between 2^9 and 2^15: what a weight loses is 2^-34 of the largest, a million keys together 2^-14 of it
+// (weights of at most one would lose 2^-25 each, and sums over many keys count on them).  Lags of
+// 8, 6 and 4 (what is left of 15) take 101, 103 and 111 us for 32 requests of 1 ... 64 new tokens behind 4096
+// keys, 100 before the weights were raised: each move rescales O.
+template <bool BF16>
+struct WeightRange {
+  static constexpr float kBelow = BF16 ? 0.f : 9.f, kReach = BF16 ? 8.f : 15.f;
+};
 
 // A part of a row's softmax that another launch joins: out / l and lse in base 2.
 struct Partials {
@@ -590,9 +600,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
           keep[i] = 1.f;
-          if (top > m[n][i] + kLazy) {
-            keep[i] = exp2_fast(m[n][i] - top);
-            m[n][i] = top;
+          if (top > m[n][i] + WeightRange<BF16>::kReach) {
+            const float base = top - WeightRange<BF16>::kBelow;
+            keep[i] = exp2_fast(m[n][i] - base);
+            m[n][i] = base;
           }
         }
         if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
@@ -606,8 +617,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
           l[n][0] *= keep[0];
           l[n][1] *= keep[1];
         }
-        // The weights enter the second product in the element type, as a rounded part and the
-        // rounded rest: two products, error 2^-16 instead of 2^-8, on pipes that HBM leaves idle.
+        // The weights enter the second product in the element type, as a rounded part and the rounded
+        // rest: two products, error 2^-16 (bf16; fp16 2^-22, and 2^-34 of the largest) instead of 2^-8,
+        // on pipes that HBM leaves idle.
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float w0 = exp2_fast(s[n][2 * i] - (m[n][0] == -INFINITY ? 0.f : m[n][0]));
@@ -786,10 +798,12 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
 // for 42 % of the active cycles in the 16-tile pieces of a prefix (start, Q, first S and O's way out).
 //
 // The maximum is only moved (and O rescaled in tensor memory, by the softmax threads) when it
-// grows by more than 8 in base 2: P and l may exceed 1 by that factor, which fp32 sums and 16-bit P hold.
+// grows by more than 8 in base 2 (6 in fp16, see WeightRange): fp32 sums and 16-bit P hold the factor.
 // S of the next tile overwrites P: it is issued behind the PV that reads it, and the commit behind
 // it tells the softmax warps that this PV, too, is complete.  P is rounded to the element type
-// (half a step, 2^-8 in bf16): the tensor cores take no wider second operand.
+// (half a step: 2^-8 in bf16; in fp16 2^-11, and 2^-34 of the largest for small weights): the rest, as a
+// second operand, would double the products of PV, which bound this kernel.  l sums the weights before
+// they are rounded.
 //
 // Pages of 8 to 128 keys (powers of two) and of multiples of 128 are loaded by TMA, one box a page
 // and 64-element half row, 128-byte swizzled; a tile that reaches past the last key, and other page
@@ -1212,11 +1226,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
           for (int e = 0; e < 4; ++e) tops[e] = max3(tops[e], s[kKeys - 4 + e], tops[0]);
           float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]);
           top = top == -INFINITY ? top : top * scale2;
-          if (__any_sync(0xffffffffu, !(top <= m + kLazy))) {
+          constexpr float kBelow = WeightRange<BF16>::kBelow, kReach = WeightRange<BF16>::kReach;
+          if (__any_sync(0xffffffffu, !(top <= m + kReach))) {
             float keep = 1.f;
-            if (!(top <= m + kLazy)) {  // a NaN score, too, moves it: the row is NaN from here on
-              keep = exp2_fast(m - top);
-              m = top;
+            if (!(top <= m + kReach)) {  // a NaN score, too, moves it: the row is NaN from here on
+              keep = exp2_fast(m - (top - kBelow));
+              m = top - kBelow;
             }
             l *= keep;
             if (j > 0) {

@@ -18,6 +18,19 @@ def half_step(dtype: torch.dtype) -> float:
     return torch.finfo(dtype).eps / 2
 
 
+def weight_rounding(kind, dtype):
+    """(relative to the weight, relative to the largest one): how far the weights that a kernel
+    takes into the second product may be from ``exp(s - m)``.  ``kind``: "tiles" (several tokens a
+    request, shared prefixes) rounds them once; "single" (one token a request) feeds a rounded part
+    and the rounded rest; "rows" (head dims without matrix products) keeps them in fp32.  fp16 holds
+    them 2^9 times as large, so that the half step 2^-25 of its smallest numbers is 2^-34 of the
+    largest weight."""
+    u = half_step(dtype)
+    if kind == "rows":
+        return 0.0, 2.0 ** -126
+    return (u if kind == "tiles" else u * u), 2.0 ** (-34 if dtype == torch.float16 else -126)
+
+
 def qk_norm_rotary(x, weight, positions, cos_sin, head_dim, eps):
     """(exact, bound) of ``x`` [T, heads * head_dim] normalised by head and rotated."""
     D, E = head_dim, head_dim // 2
@@ -43,11 +56,12 @@ def _listed(indptr, indices, last, i, block_size):
 
 
 def paged_attention(query, k_cache, v_cache, own, qo_indptr=None, prefix=None, group_indptr=None,
-                    scale=None, causal=True):
+                    scale=None, causal=True, weights=None):
     """(out, out bound, lse, lse bound) in float64; rows outside qo_indptr are NaN.
 
     ``query`` [T, HQ, D]; the caches [NB, BS, H, D]; ``own`` and ``prefix`` are
-    ``(indptr, indices, last_page_len)``."""
+    ``(indptr, indices, last_page_len)``; ``weights`` what :func:`weight_rounding` gives (default: one
+    rounding to the element type, with its smallest numbers)."""
     T, HQ, D = query.shape
     BS, H = k_cache.shape[1:3]
     group = HQ // H
@@ -55,6 +69,7 @@ def paged_attention(query, k_cache, v_cache, own, qo_indptr=None, prefix=None, g
     B = len(own[2])
     first = list(range(B + 1)) if qo_indptr is None else [int(x) for x in qo_indptr]
     u = half_step(query.dtype)
+    own_step, floor = weights or (u, torch.finfo(query.dtype).smallest_normal * u)
     out = torch.full((T, HQ, D), math.nan, dtype=torch.float64)
     bound, lse, lse_bound = torch.zeros_like(out), torch.full((T, HQ), math.nan, dtype=torch.float64), torch.zeros(T, HQ, dtype=torch.float64)
 
@@ -91,9 +106,9 @@ def paged_attention(query, k_cache, v_cache, own, qo_indptr=None, prefix=None, g
             lse[t] = torch.logsumexp(s, -1)
             # the exponential (its argument rounded once more), the sums over the keys, a few joins
             sums = (seen + 64) * F32
-            weights = 2 * s_err + 2.0 ** -20 + sums
+            fp32 = 2 * s_err + 2.0 ** -20 + sums
             # weights below the normal range lose bits against the largest one
-            tiny = seen * torch.finfo(query.dtype).smallest_normal * u * v.abs().amax()
-            bound[t] = u * out[t].abs() + (u + weights[:, None]) * (1 + u) * size + tiny
+            tiny = seen * floor * v.abs().amax()
+            bound[t] = u * out[t].abs() + (own_step + fp32[:, None]) * (1 + u) * size + tiny
             lse_bound[t] = s_err + 2.0 ** -20 + sums + 4 * F32 * lse[t].abs()
     return out, bound, lse, lse_bound
