@@ -338,6 +338,10 @@ int lms_qk_norm_rope_and_cache(const lms_qk_norm_args* args, void* stream);
  * num_requests).  Its n tokens are the last n of its len keys: with causal != 0 the i-th reads the
  * keys j <= len - n + i, else all.  Query head h reads key head h / (num_heads / num_kv_heads).
  *   s_j = scale * q.k_j,  out = sum_j exp(s_j - lse) v_j,  lse = log sum_j exp(s_j)
+ * A NaN score makes its row NaN; an infinite or NaN element of a V that a row reads makes the row's
+ * element what the formula has, as long as the key's weight is 2^-126 of the row's largest at least, in
+ * fp16 2^-22 (its rest, rounded, is not 0 then); below, the element may be NaN or miss it.  What a row
+ * does not read never reaches it.
  * A row without any key gives out = 0 and lse = -inf; tokens outside [qo_indptr[0],
  * qo_indptr[num_requests]) are left as they are.
  *

@@ -35,6 +35,15 @@ __device__ __forceinline__ uint32_t down2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// Towards zero.
+template <bool BF16>
+__device__ __forceinline__ uint32_t down2_rz(float a, float b) {
+  uint32_t r;
+  if (BF16) asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  else asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+
 // Largest i in [0, n) with a[i] <= x, or -1 (a ascending).
 __device__ __forceinline__ int last_not_above(const int* a, int n, int x) {
   int lo = -1, hi = n - 1;
@@ -617,16 +626,17 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
           l[n][0] *= keep[0];
           l[n][1] *= keep[1];
         }
-        // The weights enter the second product in the element type, as a rounded part and the rounded
-        // rest: two products, error 2^-16 (bf16; fp16 2^-22, and 2^-34 of the largest) instead of 2^-8,
-        // on pipes that HBM leaves idle.
+        // The weights enter the second product in the element type, as a part and the rounded rest: two
+        // products, error 2^-15 (bf16; fp16 2^-21, and 2^-34 of the largest) instead of 2^-8, on pipes that
+        // HBM leaves idle.  The part is taken towards zero from a little less than the weight, so that
+        // the rest is positive: both products of an infinity in V have its sign, and neither is 0 * infinity.
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float w0 = exp2_fast(s[n][2 * i] - (m[n][0] == -INFINITY ? 0.f : m[n][0]));
           const float w1 = exp2_fast(s[n][2 * i + 1] - (m[n][1] == -INFINITY ? 0.f : m[n][1]));
           l[n][0] += w0;
           l[n][1] += w1;
-          const uint32_t h = down2<BF16>(w0, w1);
+          const uint32_t h = down2_rz<BF16>(w0 * (1.f - 0x1p-12f), w1 * (1.f - 0x1p-12f));
           const float2 f = up2<BF16>(h);
           hi[n][i] = transpose8x8(h);
           lo[n][i] = transpose8x8(down2<BF16>(w0 - f.x, w1 - f.y));

@@ -150,9 +150,11 @@ def paged_attention(query: torch.Tensor, paged_kv_cache: Cache, kv_indptr: torch
     reads the keys ``j <= len - n + i``, otherwise all ``len``.  ``scale`` multiplies ``q . k``
     (default ``head_dim ** -0.5``).  Returns the output in the shape of ``query``, and with
     ``return_lse`` also the natural logarithm of every row's sum of ``exp(scale q . k)``, fp32
-    ``[T, num_heads]``.  A row that reads no key is 0, its logarithm ``-inf``.  Rows outside
-    ``qo_indptr[0]:qo_indptr[-1]`` (a padded batch) are not written: pass ``out`` (same shape and
-    dtype, sharing no memory with the inputs) to say what they hold.
+    ``[T, num_heads]``.  A row that reads no key is 0, its logarithm ``-inf``.  NaN and infinities in
+    keys and values reach the rows that read them, as in the formula (an infinity whose weight is
+    below 2^-126 of the row's largest, in fp16 2^-22, may give NaN or be lost), and no other row.  Rows outside ``qo_indptr[0]:qo_indptr[-1]`` (a padded
+    batch) are not written, their logarithms neither: pass ``out`` (same shape and dtype, sharing no
+    memory with the inputs) to say what they hold.
 
     Head dims up to 256 that are multiples of 8; 64 and 128 run on the tensor cores, the others on the
     CUDA cores, which is slow for prompts.  Forward only: nothing is recorded for a gradient.

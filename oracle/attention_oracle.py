@@ -21,14 +21,14 @@ def half_step(dtype: torch.dtype) -> float:
 def weight_rounding(kind, dtype):
     """(relative to the weight, relative to the largest one): how far the weights that a kernel
     takes into the second product may be from ``exp(s - m)``.  ``kind``: "tiles" (several tokens a
-    request, shared prefixes) rounds them once; "single" (one token a request) feeds a rounded part
-    and the rounded rest; "rows" (head dims without matrix products) keeps them in fp32.  fp16 holds
-    them 2^9 times as large, so that the half step 2^-25 of its smallest numbers is 2^-34 of the
-    largest weight."""
+    request, shared prefixes) rounds them once; "single" (one token a request) feeds a part, rounded
+    towards zero from 2^-12 less than the weight, and the rest, at most a step and 2^-12 of the weight,
+    rounded; "rows" (head dims without matrix products) keeps them in fp32.  fp16 holds them 2^9 times
+    as large, so that the half step 2^-25 of its smallest numbers is 2^-34 of the largest weight."""
     u = half_step(dtype)
     if kind == "rows":
         return 0.0, 2.0 ** -126
-    return (u if kind == "tiles" else u * u), 2.0 ** (-34 if dtype == torch.float16 else -126)
+    return (u if kind == "tiles" else u * (2 * u + 2.0 ** -12)), 2.0 ** (-34 if dtype == torch.float16 else -126)
 
 
 def qk_norm_rotary(x, weight, positions, cos_sin, head_dim, eps):

@@ -117,3 +117,26 @@ def test_infinite_values_of_the_newest_tokens_of_a_long_request():
     at = [(1, n - 1, 0, 1), (1, n - 30, 0, 2), (1, n - 41, 0, 3), (1, 3, 0, 4)]
     dirty, clean = with_values(c, at, [math.inf, -math.inf, math.inf, math.inf])
     same(*call(dirty, return_lse=True), bounded(dirty, clean))
+
+
+@gpu
+@pytest.mark.parametrize("prefix", [None, [150]])
+@pytest.mark.parametrize("BS", [16, 12, 8])
+@pytest.mark.parametrize("HQ,H,D,dtype", GEOMETRY)
+@pytest.mark.parametrize("lengths", BATCHES)
+def test_infinite_values_of_single_tokens(lengths, HQ, H, D, dtype, BS, prefix):
+    c = case(lengths, HQ=HQ, H=H, D=D, dtype=dtype, BS=BS, prefix=prefix, spread=0.5)
+    n = lengths[0]
+    at = [(0, 0, 0, 3), (0, n // 2, 0, 4), (0, n // 3, 0, 5), (0, n - 1, H - 1, D - 1), (0, n - 2, 0, 6), (0, 1, 0, 6)]
+    dirty, clean = with_values(c, at, [math.inf, -math.inf, math.nan, math.inf, math.inf, -math.inf])
+    same(*call(dirty, return_lse=True), bounded(dirty, clean))
+
+
+@gpu
+@pytest.mark.parametrize("D,dtype", [(128, BF), (64, HF)])
+def test_an_infinite_value_of_a_key_that_carries_all(D, dtype):
+    """Weights that the element type holds exactly leave no rest: 0 * infinity must not come of it."""
+    for n in (1, 5, 2000):
+        c = case([n, 3], HQ=4, H=2, D=D, dtype=dtype, spread=0.0)  # equal scores: every stored weight is the same power of two
+        dirty, clean = with_values(c, [(0, n - 1, 0, 1), (1, 1, 1, 2)], [math.inf, -math.inf])
+        same(*call(dirty, return_lse=True), bounded(dirty, clean))
