@@ -175,8 +175,6 @@ def _refuse_qk_norm(query, key, value, query_weight, key_weight, positions, cos_
     for n, t in (("query_weight", query_weight), ("key_weight", key_weight)):
         if t.dtype != dtype or t.shape != (head_dim,) or not t.is_contiguous():
             raise ValueError(f"{n} must be a contiguous [head_dim] vector of the query dtype")
-    if positions.dim() != 1:
-        raise ValueError("positions must be a vector")
     if kv_cache is not None:
         _require_cuda("value", value)
         _require_cuda("kv_cache", kv_cache)
@@ -189,7 +187,7 @@ def _refuse_qk_norm(query, key, value, query_weight, key_weight, positions, cos_
             raise ValueError("kv_cache heads do not match key")
         if NB and kv_cache.stride()[1:] != (BS * H * D, H * D, D, 1):
             raise ValueError("each cache block must be contiguous")
-        if slots.dim() != 1 or slots.shape[0] != query.shape[0]:
+        if slots.numel() != query.shape[0]:
             raise ValueError("slot_mapping must have one entry per token")
     for n, t in (("key", key), ("positions", positions), ("cos_sin_cache", cos_sin_cache),
                  ("query_weight", query_weight), ("key_weight", key_weight), ("value", value),
@@ -220,9 +218,9 @@ def _qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cac
         slots = slot_mapping
         if idx >= 0:
             if isinstance(slots, torch.Tensor):
-                slots = _slots_i64(slots, query.device)
+                slots = _slots_i64(slots, query.device).reshape(-1)
             if isinstance(positions, torch.Tensor):
-                positions = positions.contiguous()
+                positions = positions.reshape(-1).contiguous()
             rc = _packer.qk_norm(_qk_norm_entry, stream, idx, query, key, value, query_weight, key_weight, positions,
                                  cos_sin_cache, head_dim, kv_cache, slots, eps, q_out, k_out)
         if rc is None:
@@ -256,6 +254,7 @@ def qk_norm_rotary_pos_emb_and_cache(query: torch.Tensor, key: torch.Tensor, val
     the same launch: rotated K and ``value`` go to ``kv_cache`` (one layer, ``[num_blocks, 2,
     block_size, H, D]``) at ``slot_mapping``, the rotated query is returned, with
     ``return_key=True`` the rotated key too.  ``slot_mapping[t] < 0`` skips the cache write of token
-    ``t``; so does a slot beyond the cache (reported by the debug checks).  Slots must be distinct."""
+    ``t``; so does a slot beyond the cache (reported by the debug checks).  A token whose position is
+    outside ``cos_sin_cache`` has its V written, not its K.  Slots must be distinct."""
     return _qk_norm(query, key, value, query_weight, key_weight, positions, cos_sin_cache, head_dim, eps,
                     kv_cache, slot_mapping, return_key)

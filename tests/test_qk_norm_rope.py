@@ -220,3 +220,26 @@ def test_cpu_tensors_are_refused():
     c = case(torch.bfloat16, T=4)
     with pytest.raises(RuntimeError, match="no CPU path"):
         call(c)
+
+
+@gpu
+@pytest.mark.parametrize("pos_dtype,slot_dtype", [(torch.int32, torch.int64), (torch.int64, torch.int32)])
+def test_positions_and_slots_of_any_shape(pos_dtype, slot_dtype):
+    """One entry a token, as the other rotary calls take them: [batch, tokens], columns of a table."""
+    from lmserve_b200.ops import rotary_pos_emb_and_cache
+    d = on_gpu(case(T=24, pos_dtype=pos_dtype))
+    want = call(d)
+    cache = d["cache"].clone()
+    table = torch.stack((d["slots"], d["slots"]), 1).to(slot_dtype)
+    for pos, slots in ((d["pos"].view(4, 6), d["slots"].view(24, 1)), (d["pos"].view(24, 1).expand(24, 2)[:, 1], table[:, 1])):
+        d["cache"].zero_()
+        rotary_pos_emb_and_cache(d["q"], d["k"], d["v"], pos, d["cs"], d["D"], d["cache"], slots)
+        got = call(dict(d, pos=pos, slots=slots))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        written = d["slots"]
+        for plane in (0, 1):
+            assert torch.equal(d["cache"][written // 16, plane, written % 16], cache[written // 16, plane, written % 16])
+    with pytest.raises(TypeError, match="one entry per token"):
+        call(dict(d, pos=d["pos"].view(4, 6)[:3]))
+    with pytest.raises(ValueError, match="one entry per token"):
+        call(dict(d, slots=d["slots"].view(4, 6)[:3]))
