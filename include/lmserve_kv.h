@@ -349,7 +349,8 @@ int lms_qk_norm_rope_and_cache(const lms_qk_norm_args* args, void* stream);
  * (group_indptr == NULL: num_groups == 1, all requests) read, before their own keys, every key of
  * the pages prefix_indices[prefix_indptr[g] .. prefix_indptr[g+1]) (last page:
  * prefix_last_page_len[g] keys).  The result is that of a page table with the prefix in front of
- * each request's own pages; the prefix's keys are read once for all rows of the group.  A request
+ * each request's own pages; with heads of 64 and 128 the prefix's keys are read once for every 256 rows
+ * (token * heads of a key head) of the group, with other head dims once a row.  A request
  * outside every group has no prefix.
  *
  * Pages: key / value cache with block_stride bytes between pages and slot_stride bytes between

@@ -251,7 +251,7 @@ struct Partials {
 // side is full of keys or head elements and the 8-wide side holds the G rows: half the products and
 // registers of the other way round for G <= 8.  S^T turns into the second product's operand with
 // movmatrix.  Measured (HBM copy rate 6.55 TB/s): 256 requests of up to 4000 keys, 8 key heads of 128,
-// 2.1 GB in 308 to 314 us (324 among other work), 6.5 to 6.7 TB/s; 512 requests of up to 1500 keys on one
+// 2.1 GB in 308 to 314 us one call behind the other, 310 to 328 among other work; 512 requests of up to 1500 keys on one
 // key head, 225 MB in 50 us, 4.5 TB/s: the first tiles are there after 4 to 5 us, the SMs' shares of the bandwidth differ by 15 %, and the
 // slowest of the equal runs decides.  What the borders between the KS parts cut is joined through shared
 // memory at the end (one barrier a CTA; a barrier a request, with the tiles dealt out in turn, cost 2 to 4 us each).
@@ -800,9 +800,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1) attention_decode_kernel(
 //   warp 10          issues the MMAs: PV of a tile, then the next QK of the same row tile, so that
 //                    one row tile's softmax runs beside the other's products
 //
-// Measured: four prompts of 1000 to 3000 tokens, 28 query on 4 key heads of 128, causal, 226 GFLOP in 211 to
-// 243 us (0.93 to 1.07 PFLOP/s of 1.66 measured for a large product; the same binary takes one or the other
-// time from process to process).  A pair of 128-key tiles takes 3000 cycles where its four products
+// Measured: four prompts of 1000 to 3000 tokens, 28 query on 4 key heads of 128, causal, 226 GFLOP in 240 to
+// 248 us (0.91 to 0.94 PFLOP/s of 1.66 measured for a large product).  A pair of 128-key tiles takes 3000 cycles where its four products
 // take 2048: the softmax of a row tile (2100) and its products (900 behind its last P) follow one another,
 // and two row tiles, all that tensor memory holds, overlap them to two thirds.  The tensor pipe is active
 // for 42 % of the active cycles in the 16-tile pieces of a prefix (start, Q, first S and O's way out).
@@ -1701,8 +1700,9 @@ long long row_tiles(long long tokens, long long seqs, const AttentionParams& p) 
   return tiles < seqs ? seqs : tiles;
 }
 
-// Splits of the keys so that the row tiles fill the GPU, a tile of keys each at least.  (Twice or three
-// times the pieces: 256 requests behind 8192 keys 108 and 114 us instead of 100.)
+// Splits of the keys so that the row tiles fill the GPU, a tile of keys each at least.  One count for all
+// sequences, from the mean of their keys by the length of the table.  (Twice or three times the pieces:
+// 256 requests behind 8192 keys, prefix and own keys one behind the other, 108 and 114 us instead of 104.)
 int splits_of(long long tokens, long long seqs, long long pages, const AttentionParams& p, int sms) {
   const long long keys = pages * p.block_size / (seqs > 0 ? seqs : 1);
   const long long tiles = row_tiles(tokens, seqs, p);
@@ -1733,8 +1733,8 @@ AttentionPlan plan_of(const AttentionParams& p, int sms) {
     if (shared) {
       // Beside the tiles of a prefix the runs take some of the SMs, and the prefix's pieces go over the
       // others in whole rounds: the pair of shares and splits that ends first, by what either takes on
-      // an SM - 0.19 us a 16-key unit of a head of 128 (43 GB/s), 1.7 us a key tile and 8 us a piece -
-      // and what the join reads.  (256 requests behind 8192 keys: 104 us one behind the other, 100 with
+      // an SM - 0.19 us a 16-key unit of a head of 128 (43 GB/s), 1.7 us a key tile and 8 us a piece,
+      // taken for other head dims too - and what the join reads.  (256 requests behind 8192 keys: 104 us one behind the other, 100 with
       // half the SMs each, 114 where the pieces leave a third round; 8 groups: 58 to 48 us.)
       const double own = (double)units * p.num_kv_heads * p.head_dim * (0.19 / 128);
       const double tiles = (double)row_tiles(p.num_tokens, p.num_groups, p) * p.num_kv_heads;

@@ -5,7 +5,7 @@
 ``params.prefill`` and ``params.decode`` hold its arguments.  There is nothing to plan: the
 kernels read the lengths from those arrays, so a call captured into a CUDA graph follows their
 contents from replay to replay.  ``shared_prefix_attention`` is the same attention for requests
-that share long prefixes, which it reads once a group instead of once a request.
+that share long prefixes, which it reads once a group instead of once a request (heads of 64 and 128).
 """
 from __future__ import annotations
 
@@ -171,7 +171,8 @@ def shared_prefix_attention(query: torch.Tensor, paged_kv_cache: Cache,
                             qo_indptr: Optional[torch.Tensor] = None,
                             scale: Optional[float] = None, causal: bool = True,
                             return_lse: bool = False, out: Optional[torch.Tensor] = None):
-    """:func:`paged_attention` for requests that share prefixes, read once for all of them.
+    """:func:`paged_attention` for requests that share prefixes, read once for all of them where the
+    head dim is 64 or 128 (once a row otherwise: right, but nothing is saved).
 
     The requests ``group_indptr[g]:group_indptr[g + 1]`` (int32; without it there is one group of
     all requests) read every key of the pages ``prefix_indices[prefix_indptr[g]:prefix_indptr[g +
