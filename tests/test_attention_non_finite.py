@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from test_paged_attention import BF, HF, call, case, exact
+from test_paged_attention import BF, HF, call, case, drawn, exact
 
 gpu = pytest.mark.gpu
 
@@ -140,3 +140,25 @@ def test_an_infinite_value_of_a_key_that_carries_all(D, dtype):
         c = case([n, 3], HQ=4, H=2, D=D, dtype=dtype, spread=0.0)  # equal scores: every stored weight is the same power of two
         dirty, clean = with_values(c, [(0, n - 1, 0, 1), (1, 1, 1, 2)], [math.inf, -math.inf])
         same(*call(dirty, return_lse=True), bounded(dirty, clean))
+
+
+@gpu
+@pytest.mark.parametrize("seed", range(24))
+def test_random_calls_with_something_not_finite(seed):
+    """A random call with NaN and infinities in queries, keys and values: read, masked, behind the last
+    keys of requests and in pages that no request has."""
+    c, kw = drawn(500 + seed)
+    g = torch.Generator().manual_seed(seed)
+    pick = lambda n: int(torch.randint(n, (1,), generator=g))
+    c["q"] = (0.5 * torch.randn(c["q"].shape, generator=g)).to(c["q"].dtype)  # no weight underflows
+    clean = dict(c)
+    T, HQ, D = c["q"].shape
+    NB, _, BS, H, _ = c["cache"].shape
+    c["q"], c["cache"] = c["q"].clone(), c["cache"].clone()
+    for _ in range(1 + T // 40):
+        c["q"][pick(T), pick(HQ), pick(D)] = math.nan
+    for _ in range(1 + NB * BS // 600):
+        c["cache"][pick(NB), 0, pick(BS), pick(H), pick(D)] = math.nan
+    for _ in range(3 + NB * BS // 100):
+        c["cache"][pick(NB), 1, pick(BS), pick(H), pick(D)] = [math.inf, -math.inf, math.nan][pick(3)]
+    same(*call(c, return_lse=True, **kw), bounded(c, clean, **kw))
